@@ -11,12 +11,17 @@ stages (ZJU-DAILY/Garfield indexsearch/):
 - ``batch_graph_search_gpu_with_prefilter_batch_process_compressed_graph_T_dataset_resident_u8``
   big_dataset_adapterV3.cuh:3719-4117 (out-of-core; the index is ``Index.create_streamed``)
 
+Beside them, on torch tensors of the GPU, the operators of learned retrieval
+(operators.py): rows at four bits with their products and gradient, and the
+routing of queries to cells.
+
 All computation runs in the HIP library; every call raises if the library has
 not been built or cannot reach a GPU, and there is no CPU fallback.
 """
 from ._lib import (GarfieldError, Index, Batch, SearchStats, BuildStats, lib_path, f2h, row_norms_f16,
                    entry_points, grid_scatter, plan_cells, quantise_i8, build_graphs, optimize_graphs, kmeans, pinned_empty, search_noalloc, NO_RESULT, NCOUNTERS,
                    VEC_F32, VEC_F16, VEC_U8, VEC_I8Q, VEC_F16_REF)
+from .operators import (MXRows, Routes, mx_quantise, mx_dequantise, mx_product, mx_product_grad, route, route_grad)
 
 
 def intersection_area_mark_little_seg_V2(batch, prefilter):
@@ -63,4 +68,5 @@ __all__ = [
     "batch_graph_search_gpu_with_prefilter_and_postfilter",
     "intersection_area_mark_little_seg_batch_process",
     "batch_graph_search_gpu_with_prefilter_batch_process_compressed_graph_T_dataset_resident_u8",
+    "MXRows", "Routes", "mx_quantise", "mx_dequantise", "mx_product", "mx_product_grad", "route", "route_grad",
 ]

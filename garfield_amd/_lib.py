@@ -89,6 +89,15 @@ class BuildStats(C.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class MXRowsStruct(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_uint64), ("K", C.c_uint32)]
+
+
+class RouteOpts(C.Structure):
+    _fields_ = [("k", C.c_uint32), ("score", C.c_int32), ("groups", C.c_uint32), ("keep_groups", C.c_uint32),
+                ("group_score", C.c_int32), ("renormalise", C.c_int32), ("scale", C.c_float)]
+
+
 _SYMBOLS = {
     "gf_index_open": [C.POINTER(_Paths), C.POINTER(_OpenOpts), C.POINTER(C.c_void_p)],
     "gf_index_create": [C.POINTER(_Host), C.POINTER(_OpenOpts), C.POINTER(C.c_void_p)],
@@ -132,6 +141,20 @@ _SYMBOLS = {
     "gf_batch_set_stream_plan": [C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p],
     "gf_batch_get_stream_plan": [C.c_void_p, C.POINTER(C.c_uint32), C.c_void_p, C.c_void_p],
     "gf_quantise_i8": [C.c_void_p, C.c_uint64, C.c_uint32, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p],
+    "gf_mx_quantise": [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint64, C.c_void_p, C.c_void_p,
+                       C.c_void_p],
+    "gf_mx_dequantise": [C.POINTER(MXRowsStruct), C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p],
+    "gf_mx_product": [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint64, C.POINTER(MXRowsStruct), C.c_int32, C.c_void_p,
+                      C.c_uint64, C.c_void_p, C.c_size_t, C.c_void_p],
+    "gf_mx_product_mx": [C.POINTER(MXRowsStruct), C.POINTER(MXRowsStruct), C.c_int32, C.c_void_p, C.c_uint64,
+                         C.c_void_p, C.c_size_t, C.c_void_p],
+    "gf_mx_product_grad": [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint64, C.POINTER(MXRowsStruct), C.c_int32,
+                           C.c_void_p, C.c_uint64, C.c_void_p, C.c_size_t, C.c_void_p],
+    "gf_mx_product_workspace": [C.c_int32, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint32, C.POINTER(C.c_size_t)],
+    "gf_route": [C.POINTER(RouteOpts), C.c_void_p, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint64, C.c_void_p,
+                 C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
+    "gf_route_grad": [C.POINTER(RouteOpts), C.c_void_p, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint64, C.c_void_p,
+                      C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p],
     "gf_host_alloc": [C.c_size_t, C.POINTER(C.c_void_p)],
     "gf_host_free": [C.c_void_p],
     "gf_status_str": [C.c_int32],

@@ -1,0 +1,309 @@
+"""Operators of learned retrieval on torch tensors of the GPU (the device-memory
+calls of include/garfield.h).
+
+- ``mx_quantise`` / ``mx_dequantise``: rows to microscaled 4-bit floating point
+  (``MXRows``) and back.
+- ``mx_product``: scores of queries, real or quantised, against such rows;
+  ``mx_product_grad`` its gradient with respect to the queries.
+- ``route``: each query's k cells (experts) from its logits; ``route_grad`` the
+  gradient with respect to the logits.
+
+``mx_product`` and ``route`` take part in autograd.  Work goes to the current
+stream of the tensors' device and nothing waits for it.  Matrices may have any
+row distance; their last dimension must be contiguous.  Every call raises if
+the library is missing; there is no other code path.
+"""
+import ctypes as C
+
+from . import _lib
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORES = {"max": 0, "top2": 1}
+_types = None
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _type(dtype, what):
+    global _types
+    if _types is None:
+        t = _torch()
+        _types = {t.float32: 0, t.float16: 1, t.bfloat16: 2}
+    code = _types.get(dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {dtype}")
+    return code
+
+
+def _matrix(x, what):
+    """x as the library reads it: (type, rows, columns, row distance)."""
+    if not isinstance(x, _torch().Tensor) or x.ndim != 2:
+        raise ValueError(f"{what} must be a matrix (a 2-d tensor)")
+    if not x.is_cuda:
+        raise ValueError(f"{what} must be on the GPU")
+    n, d = x.shape
+    if d > 1 and x.stride(1) != 1:
+        raise ValueError(f"{what}'s last dimension must be contiguous")
+    ld = x.stride(0) if n > 1 else d
+    if ld < d:
+        raise ValueError(f"{what}'s rows overlap")
+    return _type(x.dtype, what), n, d, ld
+
+
+def _vector(x, n, dtype, device, what):
+    if x is None:
+        return None
+    if x.shape != n or x.dtype != dtype or x.device != device or not x.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {tuple(n)} {dtype} tensor on {device}")
+    return x.data_ptr()
+
+
+class _On:
+    """The device and stream of a call's tensors."""
+
+    def __init__(self, device):
+        cuda = _torch().cuda
+        self.stream = cuda.current_stream(device).cuda_stream
+        self.guard = cuda.device(device) if cuda.current_device() != device.index else None
+
+    def call(self, fn, *args):
+        if self.guard is None:
+            _lib._check(fn(*args, self.stream))
+        else:
+            with self.guard:
+                _lib._check(fn(*args, self.stream))
+
+
+class MXRows:
+    """Rows at four bits: codes (rows, 64 S) and scales (rows, 4 S), uint8,
+    S = ceil(K / 128); the layout is gf_mx_rows'."""
+
+    def __init__(self, codes, scales, K):
+        torch = _torch()
+        S = -(-int(K) // 128)
+        if K < 1:
+            raise ValueError("K must be at least 1")
+        for t, width, align, what in ((codes, 64 * S, 16, "codes"), (scales, 4 * S, 4, "scales")):
+            if (not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.ndim != 2 or t.shape[1] != width
+                    or t.shape[0] != codes.shape[0] or not t.is_contiguous() or not t.is_cuda
+                    or t.device != codes.device):
+                raise ValueError(f"{what} must be a contiguous (rows, {width}) uint8 tensor on the GPU")
+            if t.data_ptr() % align:
+                raise ValueError(f"{what} must be aligned to {align} bytes")
+        self.codes, self.scales, self.K = codes, scales, int(K)
+        self._struct = _lib.MXRowsStruct(codes.data_ptr(), scales.data_ptr(), codes.shape[0], self.K)
+
+    @property
+    def rows(self):
+        return self.codes.shape[0]
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def __getitem__(self, rows):
+        """A run of whole rows (a slice of step 1), such as one cell's, without a copy."""
+        if not isinstance(rows, slice) or rows.step not in (None, 1):
+            raise TypeError("MXRows takes slices of consecutive rows")
+        return MXRows(self.codes[rows], self.scales[rows], self.K)
+
+
+def mx_quantise(x):
+    """The rows of x (n, K) at four bits (gf_mx_quantise)."""
+    torch = _torch()
+    t, n, K, ld = _matrix(x, "x")
+    if K < 1:
+        raise ValueError("x must have at least one column")
+    S = -(-K // 128)
+    codes = torch.empty((n, 64 * S), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((n, 4 * S), dtype=torch.uint8, device=x.device)
+    _On(x.device).call(_lib.load().gf_mx_quantise, x.data_ptr(), t, n, K, ld, codes.data_ptr(), scales.data_ptr())
+    return MXRows(codes, scales, K)
+
+
+def mx_dequantise(w, dtype=None):
+    """The values that w's rows stand for, (rows, K), float32 by default."""
+    torch = _torch()
+    if not isinstance(w, MXRows):
+        raise ValueError("w must be MXRows")
+    dtype = dtype or torch.float32
+    t = _type(dtype, "dtype")
+    out = torch.empty((w.rows, w.K), dtype=dtype, device=w.device)
+    _On(w.device).call(_lib.load().gf_mx_dequantise, C.byref(w._struct), t, out.data_ptr(), w.K)
+    return out
+
+
+def _workspace(kind, t, M, w):
+    n = C.c_size_t()
+    _lib._check(_lib.load().gf_mx_product_workspace(kind, t, M, w.rows, w.K, C.byref(n)))
+    if not n.value:
+        return None, 0
+    torch = _torch()
+    return torch.empty(n.value, dtype=torch.uint8, device=w.device), n.value
+
+
+def _product(x, w, dtype):
+    torch = _torch()
+    if not isinstance(w, MXRows):
+        raise ValueError("w must be MXRows")
+    lib = _lib.load()
+    if isinstance(x, MXRows):
+        if x.K != w.K or x.device != w.device:
+            raise ValueError(f"x holds {x.K} values a row on {x.device}, w {w.K} on {w.device}")
+        dtype = dtype or torch.float32
+        to = _type(dtype, "dtype")
+        out = torch.empty((x.rows, w.rows), dtype=dtype, device=w.device)
+        ws, nws = _workspace(1, 0, x.rows, w)
+        _On(w.device).call(lib.gf_mx_product_mx, C.byref(x._struct), C.byref(w._struct), to, out.data_ptr(), w.rows,
+                           ws.data_ptr() if nws else None, nws)
+        return out
+    t, M, K, ld = _matrix(x, "x")
+    if K != w.K or x.device != w.device:
+        raise ValueError(f"x holds {K} values a row on {x.device}, w {w.K} on {w.device}")
+    dtype = dtype or x.dtype
+    to = _type(dtype, "dtype")
+    out = torch.empty((M, w.rows), dtype=dtype, device=w.device)
+    ws, nws = _workspace(0, t, M, w)
+    _On(w.device).call(lib.gf_mx_product, x.data_ptr(), t, M, ld, C.byref(w._struct), to, out.data_ptr(), w.rows,
+                       ws.data_ptr() if nws else None, nws)
+    return out
+
+
+def mx_product_grad(dy, w, dtype=None):
+    """The gradient of mx_product(x, w) with respect to x, (M, K), from dy
+    (M, rows); dy's type by default (gf_mx_product_grad)."""
+    torch = _torch()
+    if not isinstance(w, MXRows):
+        raise ValueError("w must be MXRows")
+    t, M, N, ld = _matrix(dy, "dy")
+    if N != w.rows or dy.device != w.device:
+        raise ValueError(f"dy holds {N} values a row on {dy.device}, w has {w.rows} rows on {w.device}")
+    dtype = dtype or dy.dtype
+    to = _type(dtype, "dtype")
+    dx = torch.empty((M, w.K), dtype=dtype, device=w.device)
+    ws, nws = _workspace(2, t, M, w)
+    _On(w.device).call(_lib.load().gf_mx_product_grad, dy.data_ptr(), t, M, ld, C.byref(w._struct), to,
+                       dx.data_ptr(), w.K, ws.data_ptr() if nws else None, nws)
+    return dx
+
+
+_functions = None
+
+
+def _autograd():
+    """The autograd nodes, made at the first call that needs one."""
+    global _functions
+    if _functions is None:
+        torch = _torch()
+
+        class Product(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, x, w, dtype):
+                ctx.w, ctx.dtype = w, x.dtype
+                return _product(x, w, dtype)
+
+            @staticmethod
+            def backward(ctx, dy):
+                if dy.ndim == 2 and dy.shape[1] > 1 and dy.stride(1) != 1 or dy.stride(0) < dy.shape[1]:
+                    dy = dy.contiguous()
+                return mx_product_grad(dy, ctx.w, ctx.dtype), None, None
+
+        class Route(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, logits, k, bias, groups, keep_groups, group_score, score, renormalise, scale):
+                ids, weights, load = _route(logits, k, bias, groups, keep_groups, group_score, score, renormalise,
+                                            scale)
+                ctx.save_for_backward(logits, ids, bias)
+                ctx.how = dict(score=score, renormalise=renormalise, scale=scale)
+                ctx.mark_non_differentiable(ids, load)
+                return ids, weights, load
+
+            @staticmethod
+            def backward(ctx, _ids, dweights, _load):
+                logits, ids, bias = ctx.saved_tensors
+                d = route_grad(logits, ids, dweights.contiguous(), bias=bias, **ctx.how)
+                return (d,) + (None,) * 8
+
+        _functions = Product, Route
+    return _functions
+
+
+def mx_product(x, w, dtype=None):
+    """Scores (M, rows) of x against w's rows: x a matrix (M, K), whose values
+    enter unrounded, or MXRows.  dtype: the result's type (by default x's, or
+    float32 for MXRows).  Differentiable with respect to a matrix x."""
+    if not isinstance(x, MXRows) and isinstance(x, _torch().Tensor) and x.requires_grad and _torch().is_grad_enabled():
+        return _autograd()[0].apply(x, w, dtype)
+    return _product(x, w, dtype)
+
+
+class Routes:
+    """What route returns: ids (T, k) int32, best first and -1 where a row has
+    fewer live entries; weights (T, k) float32; load (E,) int32, how many rows
+    chose each entry."""
+
+    __slots__ = ("ids", "weights", "load")
+
+    def __init__(self, ids, weights, load):
+        self.ids, self.weights, self.load = ids, weights, load
+
+    def __iter__(self):
+        return iter((self.ids, self.weights, self.load))
+
+
+def _choice(table, key, what):
+    code = table.get(key)
+    if code is None:
+        raise ValueError(f"{what} must be one of {', '.join(table)}, got {key!r}")
+    return code
+
+
+def _route(logits, k, bias, groups, keep_groups, group_score, score, renormalise, scale):
+    torch = _torch()
+    t, T, E, ld = _matrix(logits, "logits")
+    opts = _lib.RouteOpts(int(k), _choice(_SCORES, score, "score"), int(groups), int(keep_groups),
+                          _choice(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalise)), float(scale))
+    b = _vector(bias, (E,), torch.float32, logits.device, "bias")
+    dev = logits.device
+    ids = torch.empty((T, max(int(k), 0)), dtype=torch.int32, device=dev)
+    weights = torch.empty((T, max(int(k), 0)), dtype=torch.float32, device=dev)
+    load = torch.empty((E,), dtype=torch.int32, device=dev)
+    _On(dev).call(_lib.load().gf_route, C.byref(opts), logits.data_ptr(), t, T, E, ld, b, ids.data_ptr(),
+                  weights.data_ptr(), load.data_ptr())
+    return ids, weights, load
+
+
+def route(logits, k, bias=None, groups=1, keep_groups=None, group_score="max", score="softmax", renormalise=True,
+          scale=1.0):
+    """The k cells (experts) of each row of logits (T, E), by softmax or
+    sigmoid score plus bias (E,), among the keep_groups best of the groups of
+    consecutive entries; entries at -inf (or NaN) are masked (gf_route).
+    Returns Routes; the weights are differentiable with respect to the logits."""
+    keep_groups = groups if keep_groups is None else keep_groups
+    args = (logits, k, bias, groups, keep_groups, group_score, score, renormalise, scale)
+    if isinstance(logits, _torch().Tensor) and logits.requires_grad and _torch().is_grad_enabled():
+        return Routes(*_autograd()[1].apply(*args))
+    return Routes(*_route(*args))
+
+
+def route_grad(logits, ids, dweights, bias=None, score="softmax", renormalise=True, scale=1.0):
+    """The gradient of route's weights with respect to the logits, (T, E) in
+    the logits' type, from dweights (T, k) float32 and route's ids; bias, score,
+    renormalise and scale as in the call of route (gf_route_grad)."""
+    torch = _torch()
+    t, T, E, ld = _matrix(logits, "logits")
+    if ids.ndim != 2:
+        raise ValueError("ids must be (T, k)")
+    k = ids.shape[1]
+    dev = logits.device
+    i = _vector(ids, (T, k), torch.int32, dev, "ids")
+    g = _vector(dweights, (T, k), torch.float32, dev, "dweights")
+    b = _vector(bias, (E,), torch.float32, dev, "bias")
+    opts = _lib.RouteOpts(k, _choice(_SCORES, score, "score"), 1, 1, 0, int(bool(renormalise)), float(scale))
+    out = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    _On(dev).call(_lib.load().gf_route_grad, C.byref(opts), logits.data_ptr(), t, T, E, ld, b, i, g, out.data_ptr(),
+                  E)
+    return out

@@ -7,7 +7,8 @@
  * point names the reference interface it replaces (file:line under
  * indexsearch/ or indexbuild/).
  *
- * Conventions: all pointers are host pointers; sizes are element counts;
+ * Conventions: all pointers are host pointers (but for the operators on device
+ * memory at the end, which say so); sizes are element counts;
  * every call returns a gf_status (0 = success) and never exits the process;
  * gf_last_error() gives a message for the last failure on the calling thread.
  * One gf_index per device; calls on one handle must be serialised by the
@@ -447,6 +448,108 @@ gf_status gf_kmeans(const void* vectors, int32_t vec_dtype, uint32_t N, uint32_t
  * Host only (no device). */
 gf_status gf_quantise_i8(const float* x, uint64_t n, uint32_t D, float alpha, float* scale /*D*/,
                          int32_t* zero /*D*/, int8_t* out /*n*D*/);
+
+/* ---- Operators of learned retrieval, on device memory ---------------------
+ *
+ * No counterpart in the reference.  Rows at four bits with their products and
+ * gradient, and the routing of queries to cells from learned scores.  Every
+ * pointer below is a device pointer unless it is marked host; a matrix is row
+ * major with the distance of its rows (in elements) given; stream is a
+ * hipStream_t of the current device (NULL: the default stream).  The calls
+ * check their arguments on the host, enqueue their kernels and return without
+ * waiting; they allocate nothing, so they can be recorded under HIP graph
+ * capture.  Outputs must not overlap inputs.  Results do not depend on what
+ * else runs: no sum is made by floating-point atomics. */
+#define GF_F32 0   /* element types */
+#define GF_F16 1
+#define GF_BF16 2
+
+/* Rows in microscaled 4-bit floating point (the OCP MX format MXFP4): 32
+ * consecutive values of a row share a scale 2^(byte - 127), byte 255 meaning
+ * that the block is NaN; a value is a sign bit over one of 0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6 (codes 0 to 7).  Row r has S = ceil(K / 128) chunks of 128 values:
+ * codes 64 S bytes from codes + r * 64 S, two a byte, the even element in the
+ * low half, and scales 4 S bytes from scales + r * 4 S.  Values beyond K are
+ * code 0, blocks wholly beyond K have scale byte 0: the products read whole
+ * chunks and rely on it.  codes must be aligned to 16 bytes, scales to 4. */
+typedef struct {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    uint64_t rows;
+    uint32_t K;
+} gf_mx_rows;
+
+/* x (rows x K, row distance ld) to codes and scales: a block's scale byte is
+ * floor(log2 max|x|) - 2 + 127, at least 0; a value is rounded to the nearest
+ * of the grid, the middle to the even code, magnitudes over 6 to 6; a block
+ * that holds an infinity or a NaN gets scale byte 255 and codes 0. */
+gf_status gf_mx_quantise(const void* x, int32_t dtype, uint64_t rows, uint32_t K, uint64_t ld, uint8_t* codes,
+                         uint8_t* scales, void* stream);
+/* The values that the rows stand for, rounded to dtype once (exact in GF_F32,
+ * and in GF_BF16 as far as its range goes). */
+gf_status gf_mx_dequantise(const gf_mx_rows* w /*host*/, int32_t dtype, void* out, uint64_t ldo, void* stream);
+
+/* out[m][n] = sum over k of x[m][k] * w[n][k]: the scores of M queries
+ * against w's rows.  x is real (M x w->K); its values enter unrounded,
+ * whatever their type, and sums are fp32.  workspace: gf_mx_product_workspace
+ * bytes (may be NULL where that is 0), aligned to 16. */
+gf_status gf_mx_product(const void* x, int32_t dtype, uint64_t M, uint64_t ldx, const gf_mx_rows* w /*host*/,
+                        int32_t out_dtype, void* out, uint64_t ldo, void* workspace, size_t workspace_bytes,
+                        void* stream);
+/* The same with x at four bits too (x->K == w->K), on the scaled matrix
+ * instructions. */
+gf_status gf_mx_product_mx(const gf_mx_rows* x /*host*/, const gf_mx_rows* w /*host*/, int32_t out_dtype, void* out,
+                           uint64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
+/* The gradient of gf_mx_product with respect to x: dx[m][k] = sum over n of
+ * dy[m][n] * w[n][k], dy M x w->rows, dx M x w->K. */
+gf_status gf_mx_product_grad(const void* dy, int32_t dtype, uint64_t M, uint64_t ldy, const gf_mx_rows* w /*host*/,
+                             int32_t out_dtype, void* dx, uint64_t ldo, void* workspace, size_t workspace_bytes,
+                             void* stream);
+/* Workspace of the three calls above for M rows of x (or dy) against `rows`
+ * rows of K values; kind 0 gf_mx_product, 1 gf_mx_product_mx, 2
+ * gf_mx_product_grad; dtype as the call's (unused for kind 1).  Host only. */
+gf_status gf_mx_product_workspace(int32_t kind, int32_t dtype, uint64_t M, uint64_t rows, uint32_t K,
+                                  size_t* bytes /*host*/);
+
+/* Routing of T queries (tokens) to k of E cells (experts) each.  An entry is
+ * live when its logit, and its bias if there is one, is neither -inf nor NaN
+ * (a logit of +inf counts as the largest finite one).  Scores are the softmax
+ * over a row's live logits, or their sigmoids.  Entries are ranked by score +
+ * bias, compared as in exact arithmetic (64 bits), ties to the lower index;
+ * with neither a bias nor GF_GROUP_TOP2 by the logit itself.  With groups > 1
+ * (E / groups consecutive entries each) only the keep_groups best groups are
+ * ranked, a group's rank being its best entry's or the sum of its two best
+ * entries' (its only live entry's, where there is one). */
+#define GF_SCORE_SOFTMAX 0
+#define GF_SCORE_SIGMOID 1
+#define GF_GROUP_MAX 0
+#define GF_GROUP_TOP2 1
+#define GF_ROUTE_MAX_E 1024
+#define GF_ROUTE_MAX_K 64
+#define GF_ROUTE_MAX_GROUPS 64
+typedef struct {
+    uint32_t k;            /* entries a row, 1..64, at most keep_groups * E / groups */
+    int32_t score;         /* GF_SCORE_* */
+    uint32_t groups;       /* 1..64, divides E */
+    uint32_t keep_groups;  /* 1..groups */
+    int32_t group_score;   /* GF_GROUP_* */
+    int32_t renormalise;   /* weights divided by their sum over the row */
+    float scale;           /* factor of the weights */
+} gf_route_opts;
+
+/* ids, weights: T x k, best first; a row with fewer live entries ends in ids
+ * -1 of weight 0.  Weights never include the bias.  load (may be NULL): E
+ * counts of the rows that chose each entry.  E up to 1024. */
+gf_status gf_route(const gf_route_opts* opts /*host*/, const void* logits, int32_t dtype, uint64_t T, uint32_t E,
+                   uint64_t ld, const float* bias /*E or NULL*/, int32_t* ids, float* weights, int32_t* load,
+                   void* stream);
+/* The gradient of gf_route's weights with respect to the logits, the choice
+ * taken as given: dlogits (T x E, the logits' type) from dweights (T x k) and
+ * gf_route's ids.  Reads opts' k, score, renormalise and scale.  An id outside
+ * 0..E-1 has no gradient. */
+gf_status gf_route_grad(const gf_route_opts* opts /*host*/, const void* logits, int32_t dtype, uint64_t T, uint32_t E,
+                        uint64_t ld, const float* bias /*E or NULL*/, const int32_t* ids, const float* dweights,
+                        void* dlogits, uint64_t ldd, void* stream);
 
 const char* gf_status_str(gf_status s);
 const char* gf_last_error(void);
