@@ -1,39 +1,10 @@
 // Rows in microscaled 4-bit floating point: quantisation, products, gradient
 // (gfx950, wave64).  The format and its layout are described at gf_mx_rows.
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
-#include <hip/hip_runtime.h>
-
-#include "gf_operators.h"
+#include "gf_mx_device.h"
 
 namespace gf {
 namespace {
 
-template <int DT>
-struct Elem;
-template <>
-struct Elem<GF_F32> {
-    using T = float;
-    static __device__ __forceinline__ float get(T v) { return v; }
-    static __device__ __forceinline__ T put(float v) { return v; }
-};
-template <>
-struct Elem<GF_F16> {
-    using T = _Float16;
-    static __device__ __forceinline__ float get(T v) { return float(v); }
-    static __device__ __forceinline__ T put(float v) { return T(v); }
-};
-template <>
-struct Elem<GF_BF16> {
-    using T = __bf16;
-    static __device__ __forceinline__ float get(T v) { return float(v); }
-    static __device__ __forceinline__ T put(float v) { return T(v); }
-};
-
-__device__ __forceinline__ float scale_of(uint32_t byte) {
-    // 2^(byte - 127); byte 0 is the subnormal 2^-127, byte 255 NaN
-    return byte == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(byte ? byte << 23 : 1u << 22);
-}
 __device__ __forceinline__ float code_value(uint32_t c) {
     const uint32_t m = c & 7u;
     const float v = m < 2u ? 0.5f * float(m) : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
@@ -54,7 +25,7 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
 
 // One thread a block of 32 values.
 template <int DT>
-__global__ __launch_bounds__(256) void k_mx_quantise(const typename Elem<DT>::T* x, uint64_t rows, uint32_t K,
+__global__ __launch_bounds__(256) void k_mx_quantise(const ElemT<DT>* x, uint64_t rows, uint32_t K,
                                                      uint64_t ld, uint32_t nb, uint8_t* codes, uint8_t* scales) {
     const uint64_t i = uint64_t(blockIdx.x) * 256u + threadIdx.x;
     if (i >= rows * nb) return;
@@ -63,7 +34,7 @@ __global__ __launch_bounds__(256) void k_mx_quantise(const typename Elem<DT>::T*
     float v[32];
     uint32_t top = 0;
     for (uint32_t j = 0; j < 32u; ++j) {
-        v[j] = k0 + j < K ? Elem<DT>::get(x[r * ld + k0 + j]) : 0.0f;
+        v[j] = k0 + j < K ? float(x[r * ld + k0 + j]) : 0.0f;
         top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
     }
     const uint32_t byte = scale_byte(top);
@@ -79,14 +50,14 @@ __global__ __launch_bounds__(256) void k_mx_quantise(const typename Elem<DT>::T*
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void k_mx_dequantise(gf_mx_rows w, uint32_t nb, typename Elem<DT>::T* out, uint64_t ld) {
+__global__ __launch_bounds__(256) void k_mx_dequantise(gf_mx_rows w, uint32_t nb, ElemT<DT>* out, uint64_t ld) {
     const uint64_t i = uint64_t(blockIdx.x) * 256u + threadIdx.x;
     if (i >= w.rows * nb) return;
     const uint64_t r = i / nb;
     const uint32_t k0 = uint32_t(i % nb) * 32u;
-    const float s = scale_of(w.scales[i]);
+    const float s = mx_scale(w.scales[i]);
     for (uint32_t j = 0; j < 32u && k0 + j < w.K; ++j)
-        out[r * ld + k0 + j] = Elem<DT>::put(code_value(w.codes[i * 16u + j / 2u] >> (j % 2u * 4u) & 15u) * s);
+        out[r * ld + k0 + j] = ElemT<DT>(code_value(w.codes[i * 16u + j / 2u] >> (j % 2u * 4u) & 15u) * s);
 }
 
 // Element k of row r.
@@ -95,20 +66,20 @@ struct FromRows {
     uint32_t nb;
     __device__ __forceinline__ float operator()(uint64_t r, uint32_t k) const {
         const uint64_t b = r * nb + k / 32u;
-        return code_value(w.codes[b * 16u + k % 32u / 2u] >> (k % 2u * 4u) & 15u) * scale_of(w.scales[b]);
+        return code_value(w.codes[b * 16u + k % 32u / 2u] >> (k % 2u * 4u) & 15u) * mx_scale(w.scales[b]);
     }
 };
 template <int DT>
 struct FromMatrix {
-    const typename Elem<DT>::T* p;
+    const ElemT<DT>* p;
     uint64_t ld;
-    __device__ __forceinline__ float operator()(uint64_t r, uint32_t k) const { return Elem<DT>::get(p[r * ld + k]); }
+    __device__ __forceinline__ float operator()(uint64_t r, uint32_t k) const { return float(p[r * ld + k]); }
 };
 
 // out[m][n] = sum over j < J of A(m, j) * B, B = w(n, j), or w(j, n) with TR.
 template <class A, int OT, bool TR>
 __global__ __launch_bounds__(256) void k_mx_product(A a, FromRows w, uint32_t M, uint32_t N, uint32_t J,
-                                                    typename Elem<OT>::T* out, uint64_t ldo) {
+                                                    ElemT<OT>* out, uint64_t ldo) {
     __shared__ float sa[16][17], sb[16][17];
     const uint32_t tx = threadIdx.x & 15u, ty = threadIdx.x >> 4;
     const uint64_t m0 = uint64_t(blockIdx.y) * 16u, n0 = uint64_t(blockIdx.x) * 16u;
@@ -123,14 +94,7 @@ __global__ __launch_bounds__(256) void k_mx_product(A a, FromRows w, uint32_t M,
         for (uint32_t j = 0; j < 16u; ++j) acc = fmaf(sa[ty][j], sb[tx][j], acc);
         __syncthreads();
     }
-    if (m0 + ty < M && n0 + tx < N) out[(m0 + ty) * ldo + n0 + tx] = Elem<OT>::put(acc);
-}
-
-template <class F>
-hipError_t by_type(int32_t dtype, F&& f) {
-    if (dtype == GF_F32) return f(std::integral_constant<int, GF_F32>());
-    if (dtype == GF_F16) return f(std::integral_constant<int, GF_F16>());
-    return f(std::integral_constant<int, GF_BF16>());
+    if (m0 + ty < M && n0 + tx < N) out[(m0 + ty) * ldo + n0 + tx] = ElemT<OT>(acc);
 }
 
 template <bool TR, class A>
@@ -138,7 +102,7 @@ hipError_t product(A a, const gf_mx_rows& w, uint32_t M, uint32_t N, uint32_t J,
     return by_type(out.dtype, [&](auto ot) {
         constexpr int OT = decltype(ot)::value;
         hipLaunchKernelGGL((k_mx_product<A, OT, TR>), dim3((N + 15u) / 16u, (M + 15u) / 16u), 256, 0, st, a,
-                           FromRows{w, 4u * mx_chunks(w.K)}, M, N, J, static_cast<typename Elem<OT>::T*>(out.p), out.ld);
+                           FromRows{w, 4u * mx_chunks(w.K)}, M, N, J, static_cast<ElemT<OT>*>(out.p), out.ld);
         return hipGetLastError();
     });
 }
@@ -150,7 +114,7 @@ hipError_t launch_mx_quantise(const MatIn& x, uint32_t K, uint8_t* codes, uint8_
     return by_type(x.dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         hipLaunchKernelGGL(k_mx_quantise<DT>, dim3(uint32_t((x.rows * nb + 255u) / 256u)), 256, 0, st,
-                           static_cast<const typename Elem<DT>::T*>(x.p), x.rows, K, x.ld, nb, codes, scales);
+                           static_cast<const ElemT<DT>*>(x.p), x.rows, K, x.ld, nb, codes, scales);
         return hipGetLastError();
     });
 }
@@ -160,7 +124,7 @@ hipError_t launch_mx_dequantise(const gf_mx_rows& w, const MatOut& out, hipStrea
     return by_type(out.dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         hipLaunchKernelGGL(k_mx_dequantise<DT>, dim3(uint32_t((w.rows * nb + 255u) / 256u)), 256, 0, st, w, nb,
-                           static_cast<typename Elem<DT>::T*>(out.p), out.ld);
+                           static_cast<ElemT<DT>*>(out.p), out.ld);
         return hipGetLastError();
     });
 }
@@ -168,19 +132,15 @@ hipError_t launch_mx_dequantise(const gf_mx_rows& w, const MatOut& out, hipStrea
 hipError_t launch_mx_product(const MatIn& x, const gf_mx_rows& w, const MatOut& out, void*, hipStream_t st) {
     return by_type(x.dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        return product<false>(FromMatrix<DT>{static_cast<const typename Elem<DT>::T*>(x.p), x.ld}, w, uint32_t(x.rows),
+        return product<false>(FromMatrix<DT>{static_cast<const ElemT<DT>*>(x.p), x.ld}, w, uint32_t(x.rows),
                               uint32_t(w.rows), w.K, out, st);
     });
-}
-
-hipError_t launch_mx_product_mx(const gf_mx_rows& x, const gf_mx_rows& w, const MatOut& out, void*, hipStream_t st) {
-    return product<false>(FromRows{x, 4u * mx_chunks(x.K)}, w, uint32_t(x.rows), uint32_t(w.rows), w.K, out, st);
 }
 
 hipError_t launch_mx_product_grad(const MatIn& dy, const gf_mx_rows& w, const MatOut& dx, void*, hipStream_t st) {
     return by_type(dy.dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        return product<true>(FromMatrix<DT>{static_cast<const typename Elem<DT>::T*>(dy.p), dy.ld}, w,
+        return product<true>(FromMatrix<DT>{static_cast<const ElemT<DT>*>(dy.p), dy.ld}, w,
                              uint32_t(dy.rows), w.K, uint32_t(w.rows), dx, st);
     });
 }

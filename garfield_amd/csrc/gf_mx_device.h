@@ -1,0 +1,112 @@
+// Device code shared by the kernels on 4-bit rows (gf_mx*.hip).
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "gf_operators.h"
+
+namespace gf {
+namespace {
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<GF_F32> {
+    using T = float;
+};
+template <>
+struct Elem<GF_F16> {
+    using T = _Float16;
+};
+template <>
+struct Elem<GF_BF16> {
+    using T = __bf16;
+};
+template <int DT>
+using ElemT = typename Elem<DT>::T;
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// 2^(byte - 127); byte 0 is the subnormal 2^-127, byte 255 NaN.
+__device__ __forceinline__ float mx_scale(uint32_t byte) {
+    return __uint_as_float(byte == 255u ? 0x7FC00000u : byte ? byte << 23 : 1u << 22);
+}
+
+// 16 bytes at an address aligned to an element only.
+struct __attribute__((packed, aligned(1))) Bytes16 {
+    uint4 v;
+};
+__device__ __forceinline__ uint4 load16(const void* p) { return static_cast<const Bytes16*>(p)->v; }
+__device__ __forceinline__ void store16(void* p, uint4 v) { static_cast<Bytes16*>(p)->v = v; }
+
+// Workgroups go to the eight XCDs in turn, each with an L2 of its own: ids are
+// dealt so that an XCD works on a run of consecutive tiles.
+__device__ __forceinline__ uint32_t xcd_run(uint32_t b, uint32_t n) {
+    const uint32_t x = b & 7u, per = n >> 3, rem = n & 7u;
+    return x * per + min(x, rem) + (b >> 3);
+}
+// Tile t of a grid of tm x tn, in bands of `band` rows of tiles, each walked
+// column by column: the tiles in flight share rows of both operands.
+__device__ __forceinline__ void tile_of(uint32_t t, uint32_t tm, uint32_t tn, uint32_t band, uint32_t& m, uint32_t& n) {
+    const uint32_t per = band * tn, g = t / per, r = t % per, h = min(band, tm - g * band);
+    m = g * band + r % h;
+    n = r / h;
+}
+
+// A wave's 32 x 64 piece of a result, from four consecutive columns a lane
+// (put: row, column, four values) to 16-byte stores of whole rows, through
+// kPieceBytes of LDS that only this wave uses.
+template <int OT>
+struct Piece {
+    using T = ElemT<OT>;
+    static constexpr uint32_t kPitch = 64u * sizeof(T) + 16u;
+    static constexpr uint32_t kBytes = 32u * kPitch;
+    static __device__ __forceinline__ void put(uint8_t* lds, uint32_t row, uint32_t col, f32x4 v) {
+        T* p = reinterpret_cast<T*>(lds + row * kPitch) + col;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 o;
+        for (int i = 0; i < 4; ++i) o[i] = T(v[i]);
+        *reinterpret_cast<T4*>(p) = o;
+    }
+    // Rows m0.. and columns n0.. of out, M x N.
+    static __device__ __forceinline__ void flush(const uint8_t* lds, T* out, uint64_t ldo, uint32_t m0, uint32_t n0,
+                                                 uint32_t M, uint32_t N) {
+        constexpr uint32_t V = 16u / sizeof(T), per = 64u / V;   // elements a store, stores a row
+        const uint32_t lane = threadIdx.x & 63u, c = lane % per * V;
+        for (uint32_t r = lane / per; r < 32u; r += 64u / per) {
+            const uint4 v = *reinterpret_cast<const uint4*>(lds + r * kPitch + c * sizeof(T));
+            if (m0 + r >= M || n0 + c >= N) continue;
+            T* p = out + uint64_t(m0 + r) * ldo + n0 + c;
+            if (n0 + c + V <= N) {
+                store16(p, v);
+            } else {
+                const T* e = reinterpret_cast<const T*>(&v);
+                for (uint32_t i = 0; i < V; ++i)
+                    if (n0 + c + i < N) p[i] = e[i];
+            }
+        }
+    }
+};
+// Orders a wave's own LDS writes before its reads by other lanes.
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <class F>
+hipError_t by_type(int32_t dtype, F&& f) {
+    if (dtype == GF_F32) return f(std::integral_constant<int, GF_F32>());
+    if (dtype == GF_F16) return f(std::integral_constant<int, GF_F16>());
+    return f(std::integral_constant<int, GF_BF16>());
+}
+
+}  // namespace
+}  // namespace gf
