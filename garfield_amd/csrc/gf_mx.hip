@@ -1,63 +1,158 @@
 // Rows in microscaled 4-bit floating point: quantisation, products, gradient
 // (gfx950, wave64).  The format and its layout are described at gf_mx_rows.
+#include <algorithm>
+
 #include "gf_mx_device.h"
 
 namespace gf {
 namespace {
 
-__device__ __forceinline__ float code_value(uint32_t c) {
-    const uint32_t m = c & 7u;
-    const float v = m < 2u ? 0.5f * float(m) : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-    return c & 8u ? -v : v;
-}
-__device__ __forceinline__ uint32_t code_of(float v) {
-    const float a = fabsf(v);
-    const uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-    return c | (__float_as_uint(v) >> 31) << 3;
-}
-// The scale byte of a block whose magnitudes' largest bit pattern is top:
-// floor(log2) is the exponent field - 127 (subnormals fall to byte 0 anyway),
-// 2 less for the grid's largest binade.
+// ---- quantisation ---------------------------------------------------------
+// Both directions are bound by memory.  A lane holds 16 bytes of the real side
+// (V = 4 or 8 values), so 8 or 4 lanes share a block and 32 or 16 a chunk of
+// 128 values; kAhead chunks a lane are loaded before the first is used.
+
+constexpr uint32_t kAhead = 4;
+
+// The scale byte of a block whose magnitudes' largest bit pattern (fp32) is
+// top: floor(log2) is the exponent field - 127 (a subnormal's is below the
+// least scale anyway), 2 less for the grid's largest binade.
 __device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
     const uint32_t e = top >> 23;
     return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
 }
 
-// One thread a block of 32 values.
+// Chunks (row, s) of a grid-strided walk; the division by S is done once.
+struct Walk {
+    uint64_t row;
+    uint32_t s;
+    uint64_t drow;
+    uint32_t ds, S;
+    __device__ __forceinline__ Walk(uint64_t first, uint64_t step, uint32_t chunks) : S(chunks) {
+        row = first / S, s = uint32_t(first % S);
+        drow = step / S, ds = uint32_t(step % S);
+    }
+    __device__ __forceinline__ void next() {
+        row += drow, s += ds;
+        if (s >= S) s -= S, ++row;
+    }
+};
+
 template <int DT>
-__global__ __launch_bounds__(256) void k_mx_quantise(const ElemT<DT>* x, uint64_t rows, uint32_t K,
-                                                     uint64_t ld, uint32_t nb, uint8_t* codes, uint8_t* scales) {
-    const uint64_t i = uint64_t(blockIdx.x) * 256u + threadIdx.x;
-    if (i >= rows * nb) return;
-    const uint64_t r = i / nb;
-    const uint32_t k0 = uint32_t(i % nb) * 32u;
-    float v[32];
-    uint32_t top = 0;
-    for (uint32_t j = 0; j < 32u; ++j) {
-        v[j] = k0 + j < K ? float(x[r * ld + k0 + j]) : 0.0f;
-        top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+__global__ __launch_bounds__(256) void k_mx_quantise(const ElemT<DT>* x, uint64_t rows, uint32_t K, uint64_t ld, uint32_t S,
+                                                     uint8_t* codes, uint8_t* scales) {
+    using T = ElemT<DT>;
+    constexpr uint32_t V = 16u / sizeof(T), kLanes = 128u / V, kChunks = 256u / kLanes;
+    const uint32_t lane = threadIdx.x % kLanes;
+    Walk at(uint64_t(blockIdx.x) * kChunks + threadIdx.x / kLanes, uint64_t(gridDim.x) * kChunks, S);
+    while (at.row < rows) {   // a chunk's lanes agree on this
+        uint4 raw[kAhead];
+        Walk w = at;
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u, w.next()) {
+            const uint32_t k = w.s * 128u + lane * V;
+            raw[u] = make_uint4(0, 0, 0, 0);
+            if (w.row >= rows) continue;
+            const T* p = x + w.row * ld + k;
+            if (k + V <= K) {
+                raw[u] = load16(p);
+            } else {
+                T t[V];
+#pragma unroll
+                for (uint32_t i = 0; i < V; ++i) t[i] = k + i < K ? p[i] : T(0.0f);
+                __builtin_memcpy(&raw[u], t, 16);
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u, at.next()) {
+            T t[V];
+            __builtin_memcpy(t, &raw[u], 16);
+            float v[V];
+            uint32_t top = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) {
+                v[i] = float(t[i]);
+                top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+            }
+            top = max(top, uint32_t(__builtin_amdgcn_mov_dpp(int(top), 0xB1, 0xF, 0xF, true)));   // lane ^ 1
+            top = max(top, uint32_t(__builtin_amdgcn_mov_dpp(int(top), 0x4E, 0xF, 0xF, true)));   // lane ^ 2
+            if (V == 4) top = max(top, uint32_t(__builtin_amdgcn_mov_dpp(int(top), 0x141, 0xF, 0xF, true)));   // 7 - lane
+            const uint32_t byte = scale_byte(top);
+            const float scale = mx_scale(byte == 255u ? 127u : byte);
+            uint32_t c = 0;
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], scale, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], scale, 1);
+            if constexpr (V == 8) {
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], scale, 2);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], scale, 3);
+            }
+            if (byte == 255u) c = 0;
+            if (at.row >= rows) continue;
+            const uint64_t chunk = at.row * S + at.s;
+            if constexpr (V == 8)
+                reinterpret_cast<uint32_t*>(codes)[chunk * 16u + lane] = c;
+            else
+                reinterpret_cast<uint16_t*>(codes)[chunk * 32u + lane] = uint16_t(c);
+            if (lane % (32u / V) == 0) scales[chunk * 4u + lane / (32u / V)] = uint8_t(byte);
+        }
     }
-    const uint32_t byte = scale_byte(top);
-    const float inv = __uint_as_float((254u - min(byte, 253u)) << 23);
-    uint32_t w[4];
-    for (uint32_t q = 0; q < 4u; ++q) {
-        w[q] = 0;
-        for (uint32_t j = 0; j < 8u; ++j)
-            if (byte != 255u) w[q] |= code_of(v[q * 8u + j] * inv) << (4u * j);
-    }
-    reinterpret_cast<uint4*>(codes)[i] = make_uint4(w[0], w[1], w[2], w[3]);
-    scales[i] = uint8_t(byte);
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void k_mx_dequantise(gf_mx_rows w, uint32_t nb, ElemT<DT>* out, uint64_t ld) {
-    const uint64_t i = uint64_t(blockIdx.x) * 256u + threadIdx.x;
-    if (i >= w.rows * nb) return;
-    const uint64_t r = i / nb;
-    const uint32_t k0 = uint32_t(i % nb) * 32u;
-    const float s = mx_scale(w.scales[i]);
-    for (uint32_t j = 0; j < 32u && k0 + j < w.K; ++j)
-        out[r * ld + k0 + j] = ElemT<DT>(code_value(w.codes[i * 16u + j / 2u] >> (j % 2u * 4u) & 15u) * s);
+__global__ __launch_bounds__(256) void k_mx_dequantise(gf_mx_rows w, uint32_t S, ElemT<DT>* out, uint64_t ld) {
+    using T = ElemT<DT>;
+    constexpr uint32_t V = 16u / sizeof(T), kLanes = 128u / V, kChunks = 256u / kLanes;
+    const uint32_t lane = threadIdx.x % kLanes;
+    Walk at(uint64_t(blockIdx.x) * kChunks + threadIdx.x / kLanes, uint64_t(gridDim.x) * kChunks, S);
+    while (at.row < w.rows) {
+        uint32_t c[kAhead], sc[kAhead];
+        Walk a = at;
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u, a.next()) {
+            const uint64_t chunk = min(a.row, w.rows - 1u) * S + a.s;
+            if constexpr (V == 8)
+                c[u] = reinterpret_cast<const uint32_t*>(w.codes)[chunk * 16u + lane];
+            else
+                c[u] = reinterpret_cast<const uint16_t*>(w.codes)[chunk * 32u + lane];
+            sc[u] = w.scales[chunk * 4u + lane / (32u / V)];
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u, at.next()) {
+            if (at.row >= w.rows) continue;
+            const float scale = mx_scale(sc[u]);
+            float v[V];
+            auto two = [&](uint32_t i, auto sel) {
+                const f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], scale, decltype(sel)::value);
+                v[i] = p[0], v[i + 1] = p[1];
+            };
+            two(0, std::integral_constant<int, 0>());
+            two(2, std::integral_constant<int, 1>());
+            if constexpr (V == 8) {
+                two(4, std::integral_constant<int, 2>());
+                two(6, std::integral_constant<int, 3>());
+            }
+            T t[V];
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) t[i] = T(v[i]);
+            const uint32_t k = at.s * 128u + lane * V;
+            T* p = out + at.row * ld + k;
+            if (k + V <= w.K) {
+                uint4 q;
+                __builtin_memcpy(&q, t, 16);
+                store16(p, q);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < V; ++i)
+                    if (k + i < w.K) p[i] = t[i];
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float code_value(uint32_t c) {
+    const uint32_t m = c & 7u;
+    const float v = m < 2u ? 0.5f * float(m) : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
+    return c & 8u ? -v : v;
 }
 
 // Element k of row r.
@@ -109,21 +204,30 @@ hipError_t product(A a, const gf_mx_rows& w, uint32_t M, uint32_t N, uint32_t J,
 
 }  // namespace
 
+namespace {
+// Workgroups for a walk over rows x S chunks, 256 threads of kAhead 16-byte
+// pieces each: one turn where they fit the grid.
+uint32_t walk_blocks(uint64_t rows, uint32_t S, uint32_t elem) {
+    const uint64_t per = 256u / (128u * elem / 16u) * kAhead;
+    return uint32_t(std::min<uint64_t>((rows * S + per - 1u) / per, 1u << 20));
+}
+}  // namespace
+
 hipError_t launch_mx_quantise(const MatIn& x, uint32_t K, uint8_t* codes, uint8_t* scales, hipStream_t st) {
-    const uint32_t nb = 4u * mx_chunks(K);
+    const uint32_t S = mx_chunks(K);
     return by_type(x.dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        hipLaunchKernelGGL(k_mx_quantise<DT>, dim3(uint32_t((x.rows * nb + 255u) / 256u)), 256, 0, st,
-                           static_cast<const ElemT<DT>*>(x.p), x.rows, K, x.ld, nb, codes, scales);
+        hipLaunchKernelGGL(k_mx_quantise<DT>, dim3(walk_blocks(x.rows, S, sizeof(ElemT<DT>))), 256, 0, st,
+                           static_cast<const ElemT<DT>*>(x.p), x.rows, K, x.ld, S, codes, scales);
         return hipGetLastError();
     });
 }
 
 hipError_t launch_mx_dequantise(const gf_mx_rows& w, const MatOut& out, hipStream_t st) {
-    const uint32_t nb = 4u * mx_chunks(w.K);
+    const uint32_t S = mx_chunks(w.K);
     return by_type(out.dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        hipLaunchKernelGGL(k_mx_dequantise<DT>, dim3(uint32_t((w.rows * nb + 255u) / 256u)), 256, 0, st, w, nb,
+        hipLaunchKernelGGL(k_mx_dequantise<DT>, dim3(walk_blocks(w.rows, S, sizeof(ElemT<DT>))), 256, 0, st, w, S,
                            static_cast<ElemT<DT>*>(out.p), out.ld);
         return hipGetLastError();
     });
