@@ -25,7 +25,7 @@ COMMON = [
     "-Wno-deprecated-declarations", "-I", os.path.join(ROOT, "include"),
 ]
 LIB_SOURCES = ["gf_kernels.hip", "gf_host.cpp", "gf_stream.cpp", "gf_io.cpp", "gf_build.cpp",
-               "gf_noalloc.cpp", "gf_mx.hip", "gf_mx_scaled.hip", "gf_route.hip", "gf_operators.cpp"]
+               "gf_noalloc.cpp", "gf_mx.hip", "gf_mx_scaled.hip", "gf_mx_real.hip", "gf_route.hip", "gf_operators.cpp"]
 OBJ_DIR = os.path.join(HERE, "_build")
 
 

@@ -149,59 +149,6 @@ __global__ __launch_bounds__(256) void k_mx_dequantise(gf_mx_rows w, uint32_t S,
     }
 }
 
-__device__ __forceinline__ float code_value(uint32_t c) {
-    const uint32_t m = c & 7u;
-    const float v = m < 2u ? 0.5f * float(m) : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-    return c & 8u ? -v : v;
-}
-
-// Element k of row r.
-struct FromRows {
-    gf_mx_rows w;
-    uint32_t nb;
-    __device__ __forceinline__ float operator()(uint64_t r, uint32_t k) const {
-        const uint64_t b = r * nb + k / 32u;
-        return code_value(w.codes[b * 16u + k % 32u / 2u] >> (k % 2u * 4u) & 15u) * mx_scale(w.scales[b]);
-    }
-};
-template <int DT>
-struct FromMatrix {
-    const ElemT<DT>* p;
-    uint64_t ld;
-    __device__ __forceinline__ float operator()(uint64_t r, uint32_t k) const { return float(p[r * ld + k]); }
-};
-
-// out[m][n] = sum over j < J of A(m, j) * B, B = w(n, j), or w(j, n) with TR.
-template <class A, int OT, bool TR>
-__global__ __launch_bounds__(256) void k_mx_product(A a, FromRows w, uint32_t M, uint32_t N, uint32_t J,
-                                                    ElemT<OT>* out, uint64_t ldo) {
-    __shared__ float sa[16][17], sb[16][17];
-    const uint32_t tx = threadIdx.x & 15u, ty = threadIdx.x >> 4;
-    const uint64_t m0 = uint64_t(blockIdx.y) * 16u, n0 = uint64_t(blockIdx.x) * 16u;
-    float acc = 0.0f;
-    for (uint32_t j0 = 0; j0 < J; j0 += 16u) {
-        sa[ty][tx] = m0 + ty < M && j0 + tx < J ? a(m0 + ty, j0 + tx) : 0.0f;
-        if (TR)
-            sb[tx][ty] = n0 + tx < N && j0 + ty < J ? w(j0 + ty, uint32_t(n0) + tx) : 0.0f;
-        else
-            sb[ty][tx] = n0 + ty < N && j0 + tx < J ? w(n0 + ty, j0 + tx) : 0.0f;
-        __syncthreads();
-        for (uint32_t j = 0; j < 16u; ++j) acc = fmaf(sa[ty][j], sb[tx][j], acc);
-        __syncthreads();
-    }
-    if (m0 + ty < M && n0 + tx < N) out[(m0 + ty) * ldo + n0 + tx] = ElemT<OT>(acc);
-}
-
-template <bool TR, class A>
-hipError_t product(A a, const gf_mx_rows& w, uint32_t M, uint32_t N, uint32_t J, const MatOut& out, hipStream_t st) {
-    return by_type(out.dtype, [&](auto ot) {
-        constexpr int OT = decltype(ot)::value;
-        hipLaunchKernelGGL((k_mx_product<A, OT, TR>), dim3((N + 15u) / 16u, (M + 15u) / 16u), 256, 0, st, a,
-                           FromRows{w, 4u * mx_chunks(w.K)}, M, N, J, static_cast<ElemT<OT>*>(out.p), out.ld);
-        return hipGetLastError();
-    });
-}
-
 }  // namespace
 
 namespace {
@@ -232,23 +179,5 @@ hipError_t launch_mx_dequantise(const gf_mx_rows& w, const MatOut& out, hipStrea
         return hipGetLastError();
     });
 }
-
-hipError_t launch_mx_product(const MatIn& x, const gf_mx_rows& w, const MatOut& out, void*, hipStream_t st) {
-    return by_type(x.dtype, [&](auto dt) {
-        constexpr int DT = decltype(dt)::value;
-        return product<false>(FromMatrix<DT>{static_cast<const ElemT<DT>*>(x.p), x.ld}, w, uint32_t(x.rows),
-                              uint32_t(w.rows), w.K, out, st);
-    });
-}
-
-hipError_t launch_mx_product_grad(const MatIn& dy, const gf_mx_rows& w, const MatOut& dx, void*, hipStream_t st) {
-    return by_type(dy.dtype, [&](auto dt) {
-        constexpr int DT = decltype(dt)::value;
-        return product<true>(FromMatrix<DT>{static_cast<const ElemT<DT>*>(dy.p), dy.ld}, w,
-                             uint32_t(dy.rows), w.K, uint32_t(w.rows), dx, st);
-    });
-}
-
-size_t mx_workspace(int32_t, int32_t, uint64_t, uint64_t, uint32_t) { return 0; }
 
 }  // namespace gf

@@ -61,13 +61,13 @@ __device__ __forceinline__ void tile_of(uint32_t t, uint32_t tm, uint32_t tn, ui
     n = r / h;
 }
 
-// A wave's 32 x 64 piece of a result, from four consecutive columns a lane
+// A wave's 32 x COLS piece of a result, from four consecutive columns a lane
 // (put: row, column, four values) to 16-byte stores of whole rows, through
-// kPieceBytes of LDS that only this wave uses.
-template <int OT>
+// kBytes of LDS that only this wave uses.
+template <int OT, uint32_t COLS>
 struct Piece {
     using T = ElemT<OT>;
-    static constexpr uint32_t kPitch = 64u * sizeof(T) + 16u;
+    static constexpr uint32_t kPitch = COLS * sizeof(T) + 16u;
     static constexpr uint32_t kBytes = 32u * kPitch;
     static __device__ __forceinline__ void put(uint8_t* lds, uint32_t row, uint32_t col, f32x4 v) {
         T* p = reinterpret_cast<T*>(lds + row * kPitch) + col;
@@ -79,27 +79,64 @@ struct Piece {
     // Rows m0.. and columns n0.. of out, M x N.
     static __device__ __forceinline__ void flush(const uint8_t* lds, T* out, uint64_t ldo, uint32_t m0, uint32_t n0,
                                                  uint32_t M, uint32_t N) {
-        constexpr uint32_t V = 16u / sizeof(T), per = 64u / V;   // elements a store, stores a row
-        const uint32_t lane = threadIdx.x & 63u, c = lane % per * V;
-        for (uint32_t r = lane / per; r < 32u; r += 64u / per) {
-            const uint4 v = *reinterpret_cast<const uint4*>(lds + r * kPitch + c * sizeof(T));
-            if (m0 + r >= M || n0 + c >= N) continue;
+        constexpr uint32_t V = 16u / sizeof(T), per = COLS / V, kTurns = per / 2u;   // elements a store, stores a row
+        const uint32_t lane = threadIdx.x & 63u;
+        if (m0 + 32u <= M && n0 + COLS <= N) {
+            const uint32_t c = lane % per * V, r = lane / per;
             T* p = out + uint64_t(m0 + r) * ldo + n0 + c;
-            if (n0 + c + V <= N) {
-                store16(p, v);
-            } else {
-                const T* e = reinterpret_cast<const T*>(&v);
-                for (uint32_t i = 0; i < V; ++i)
-                    if (n0 + c + i < N) p[i] = e[i];
-            }
+            uint4 v[kTurns];
+#pragma unroll
+            for (uint32_t i = 0; i < kTurns; ++i)
+                v[i] = *reinterpret_cast<const uint4*>(lds + (r + i * (64u / per)) * kPitch + c * sizeof(T));
+#pragma unroll
+            for (uint32_t i = 0; i < kTurns; ++i) store16(p + uint64_t(i * (64u / per)) * ldo, v[i]);
+        } else {
+            const uint32_t c = lane % COLS;
+            if (n0 + c < N)
+                for (uint32_t r = lane / COLS; r < 32u && m0 + r < M; r += 64u / COLS)
+                    out[uint64_t(m0 + r) * ldo + n0 + c] = reinterpret_cast<const T*>(lds + r * kPitch)[c];
         }
     }
 };
+// LDS byte address of a __shared__ object.
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+    return uint32_t(uintptr_t((const __attribute__((address_space(3))) void*)p));
+}
+// Asynchronous global-to-LDS copies: 16 bytes per active lane from base + off
+// (base wave-uniform) to LDS at lds_base + 16 x lane, lds_base wave-uniform
+// (in m0).  They count in vmcnt and the compiler does not see them (for copies
+// that it sees it waits before any LDS read): the caller waits (wait_vmcnt)
+// and synchronises before the data is read.
+__device__ __forceinline__ void lds_copy16(const uint8_t* base, uint32_t off, uint32_t lds_base) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds_base) : "memory");
+}
+// s_waitcnt vmcnt(N), the other counters unconstrained (gfx9 encoding).
+template <uint32_t N>
+__device__ __forceinline__ void wait_vmcnt() {
+    static_assert(N < 64u, "vmcnt");
+    __builtin_amdgcn_s_waitcnt(int((N & 15u) | ((N >> 4) << 14) | (7u << 4) | (15u << 8)));
+}
+// No instruction is scheduled across this point.
+__device__ __forceinline__ void sched_fence() { __builtin_amdgcn_sched_barrier(0); }
+// A barrier behind this wave's LDS accesses; it waits for no global ones.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 // Orders a wave's own LDS writes before its reads by other lanes.
 __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Compute units of the current device.
+inline uint32_t compute_units() {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+        return 256u;
+    return uint32_t(n);
 }
 
 template <class F>

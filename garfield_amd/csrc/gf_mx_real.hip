@@ -1,0 +1,473 @@
+// Products of real rows with 4-bit rows, and their gradient, on the bfloat16
+// matrix instructions.
+//
+// A value of a 4-bit row is exact in bfloat16, whose exponent range is the
+// format's, so only the real side could lose bits.  It does not: a binary16
+// value is the sum of two bfloat16 values, an fp32 value of three (truncated
+// eight bits at a time), and the product runs once over each of these planes.
+#include <algorithm>
+
+#include "gf_mx_device.h"
+
+namespace gf {
+namespace {
+
+template <int DT>
+constexpr int kPlanes = DT == GF_BF16 ? 1 : DT == GF_F16 ? 2 : 3;
+
+// The planes of eight values: the leading 8 bits, the next 8, the last.  An
+// infinity or NaN lies in the first alone; no remainder exceeds the value, so
+// none overflows.
+template <int P>
+__device__ __forceinline__ void split8(const float* v, uint4* plane) {
+    uint32_t out[P][4];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        uint32_t top[P][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float rest = v[i + k];
+            const uint32_t bits = __float_as_uint(rest);
+            const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
+            // a NaN keeps a bit of its payload in the upper half
+            top[0][k] = (bits & 0x7FFFFFFFu) > 0x7F800000u ? bits | 0x00400000u : bits;
+#pragma unroll
+            for (int p = 1; p < P; ++p) {
+                rest -= __uint_as_float((p == 1 ? bits : top[p - 1][k]) & 0xFFFF0000u);
+                top[p][k] = finite ? __float_as_uint(rest) : 0u;
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) out[p][i / 2] = top[p][0] >> 16 | (top[p][1] & 0xFFFF0000u);
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) plane[p] = make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
+}
+
+// Eight elements of a row from k on, zeros from K on, as planes.
+template <int DT>
+__device__ __forceinline__ void load_planes(const ElemT<DT>* row, uint32_t k, uint32_t K, uint4* plane) {
+    constexpr int P = kPlanes<DT>;
+    ElemT<DT> e[8];
+    if (k + 8u <= K) {
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(e) / 16u; ++i) {
+            const uint4 q = load16(reinterpret_cast<const uint8_t*>(row + k) + i * 16u);
+            __builtin_memcpy(reinterpret_cast<uint8_t*>(e) + i * 16u, &q, 16);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) e[i] = k + i < K ? row[k + i] : ElemT<DT>(0.0f);
+    }
+    if constexpr (DT == GF_BF16) {
+        __builtin_memcpy(plane, e, 16);
+    } else {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = float(e[i]);
+        split8<P>(v, plane);
+    }
+}
+
+// 8 codes to bfloat16.
+__device__ __forceinline__ bf16x8 decode8(uint32_t codes, float scale) {
+    bf16x8 o;
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1),
+                 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
+    o[0] = a[0], o[1] = a[1], o[2] = b[0], o[3] = b[1], o[4] = c[0], o[5] = c[1], o[6] = d[0], o[7] = d[1];
+    return o;
+}
+__device__ __forceinline__ bf16x8 as_bf16x8(uint4 v) {
+    bf16x8 o;
+    __builtin_memcpy(&o, &v, 16);
+    return o;
+}
+
+// ---- the real side as planes -----------------------------------------------
+// planes[p][step][row][64]: a step's 64 values of all rows together, zeros from
+// J on.
+template <int DT>
+__global__ __launch_bounds__(256) void k_mx_planes(const ElemT<DT>* x, uint64_t rows, uint32_t J, uint64_t ld, uint32_t steps,
+                                                   uint16_t* planes) {
+    const uint32_t per = steps * 8u;
+    const uint64_t n = rows * per;
+    for (uint64_t i = uint64_t(blockIdx.x) * 256u + threadIdx.x; i < n; i += uint64_t(gridDim.x) * 256u) {
+        const uint64_t r = n >> 32 ? i / per : uint32_t(i) / per;
+        const uint32_t c = uint32_t(i - r * per);
+        uint4 out[kPlanes<DT>];
+        load_planes<DT>(x + r * ld, c * 8u, J, out);
+#pragma unroll
+        for (int p = 0; p < kPlanes<DT>; ++p)
+            *reinterpret_cast<uint4*>(planes + ((uint64_t(p) * steps + c / 8u) * rows + r) * 64u + c % 8u * 8u) = out[p];
+    }
+}
+
+// ---- few queries -----------------------------------------------------------
+// Up to 16 queries: w is read once, straight to registers, and nothing else
+// counts.  A wave has 16 NT rows of w; the block's WK waves share them, each
+// with its part of K, joined in order through LDS.  Lane group g of four holds
+// block g of a chunk's four, 16 bytes; the values 8 q .. 8 q + 7 of the four
+// blocks go through one instruction, on both sides alike.
+template <int DT, int NT, int WK, int OT>
+__global__ __launch_bounds__(64 * WK) void k_mx_few(const ElemT<DT>* x, uint32_t M, uint64_t ldx, gf_mx_rows w, uint32_t S,
+                                                    ElemT<OT>* out, uint64_t ldo) {
+    constexpr int P = kPlanes<DT>;
+    __shared__ f32x4 part[WK > 1 ? WK * 64 * NT : 1];
+    const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4, wk = threadIdx.x >> 6;
+    const uint32_t N = uint32_t(w.rows), K = w.K, n0 = blockIdx.x * 16u * NT;
+    f32x4 acc[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = f32x4{0, 0, 0, 0};
+    const uint8_t *wc[NT], *ws[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {   // rows beyond the end repeat the last one; their sums are not stored
+        const uint64_t row = min(n0 + 16u * j + r, N - 1u);
+        wc[j] = w.codes + row * S * 64u + g * 16u;
+        ws[j] = w.scales + row * S * 4u + g;
+    }
+    const ElemT<DT>* xr = x + uint64_t(min(r, M - 1u)) * ldx;
+    const uint32_t s1 = uint32_t(uint64_t(S) * (wk + 1u) / WK);
+#pragma unroll 2
+    for (uint32_t s = uint32_t(uint64_t(S) * wk / WK); s < s1; ++s) {
+        uint4 c[NT], a[4][P];
+        uint32_t sc[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            c[j] = *reinterpret_cast<const uint4*>(wc[j] + uint64_t(s) * 64u);
+            sc[j] = ws[j][uint64_t(s) * 4u];
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (r < M) {
+                load_planes<DT>(xr, s * 128u + g * 32u + q * 8u, K, a[q]);
+            } else {
+#pragma unroll
+                for (int p = 0; p < P; ++p) a[q][p] = make_uint4(0, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const float scale = mx_scale(sc[j]);
+            const uint32_t word[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const bf16x8 b = decode8(word[q], scale);
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, as_bf16x8(a[q][p]), acc[j], 0, 0, 0);
+            }
+        }
+    }
+    if (WK > 1) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) part[(wk * NT + j) * 64u + lane] = acc[j];
+        __syncthreads();
+        if (wk) return;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            for (uint32_t k = 1; k < WK; ++k) acc[j] += part[(k * NT + j) * 64u + lane];
+    }
+    if (r < M) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            for (uint32_t e = 0; e < 4u; ++e) {
+                const uint32_t n = n0 + 16u * j + 4u * g + e;
+                if (n < N) out[uint64_t(r) * ldo + n] = ElemT<OT>(acc[j][e]);
+            }
+    }
+}
+
+// ---- tiles through LDS -----------------------------------------------------
+// A block has a tile of BM real rows x BN columns of the result, 64 values of
+// the sum a step, its VM x VN waves equal parts of the tile.  The real side
+// comes as planes, by copies straight to LDS, two steps ahead (three slots);
+// the 4-bit side through registers, one block of 32 values a thread, decoded
+// on its way to LDS, one step ahead (two slots).
+// Columns are rows of w (TR = false: the product) or positions in w's rows
+// (TR = true: the gradient, whose sum runs over w's rows).  Slots of the real
+// side, and of w without TR, have rows of 64 values, 128 bytes; their 16-byte
+// piece c of row r lies at place c ^ (r / 2 & 7): rows take half the banks each
+// by their parity, and of 16 rows the eight of one parity have a piece in eight
+// different places.  With TR a slot has 64 rows of BN values as they lie in w
+// and is read by the transposing LDS load, 4 rows x 16 columns a group of 16
+// lanes; the 32-byte unit u of row n lies at place u ^ (n & 3), so that the
+// four rows come from different banks.
+// The sum may be cut into `parts`, each block then writing its own in fp32 to
+// a workspace (out, rows of ldo, a part every M ldo), which k_mx_join adds up
+// in order.
+template <int BM, int BN, int OT, bool TR>
+struct RealLds {
+    static constexpr uint32_t kA = BM * 128u, kB = BN * 128u, kBytes = 3u * kA + 2u * kB;
+    static constexpr uint32_t kCols = 32u;
+    using P = Piece<OT, kCols>;
+};
+
+struct RealArgs {
+    const uint16_t* a;      // planes of the real side
+    uint64_t lda, step;     // distance of its rows and steps, in elements
+    uint32_t planes, M, J;  // J: length of the sum in steps of 64
+    gf_mx_rows w;
+    uint32_t S, N;          // N: columns of the result
+    uint32_t tm, tn, parts;
+};
+
+template <int BM, int BN, int VM, int VN, int OT, bool TR>
+__global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>* out, uint64_t ldo) {
+    using L = RealLds<BM, BN, OT, TR>;
+    using Pc = typename L::P;
+    constexpr uint32_t TH = 64u * VM * VN, kPer = BM * 8u / TH;
+    constexpr int MI = BM / VM / 32, NI = BN / VN / 32;
+    static_assert(BN * 2u == TH && VM * VN * Pc::kBytes <= L::kBytes, "");
+    __shared__ __align__(16) uint8_t lds[L::kBytes];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, r = lane & 31u, h = lane >> 5;
+    const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(tid >> 6)));
+    const uint32_t base = lds_addr(lds);
+    const uint32_t tiles = p.tm * p.tn, id = xcd_run(blockIdx.x, tiles * p.parts);
+    const uint32_t cut = id / tiles;
+    uint32_t m0, n0;
+    tile_of(id % tiles, p.tm, p.tn, 4u, m0, n0);
+    m0 *= BM, n0 *= BN;
+    const uint32_t total = p.J * p.planes;   // every plane goes over all of w
+    const uint32_t s0 = uint32_t(uint64_t(total) * cut / p.parts), s1 = uint32_t(uint64_t(total) * (cut + 1u) / p.parts);
+
+    // rows beyond the end repeat the last one; their sums are not stored
+    uint32_t oa[kPer];
+    const uint8_t* pa = reinterpret_cast<const uint8_t*>(p.a + uint64_t(m0) * p.lda);
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) {
+        const uint32_t row = i * (TH / 8u) + tid / 8u;
+        oa[i] = uint32_t(min(row, p.M - 1u - m0) * uint32_t(p.lda * 2u)) + ((tid & 7u) ^ (tid >> 4 & 7u)) * 16u;
+    }
+    auto fetch_a = [&](uint32_t s, uint32_t slot) {
+        const uint8_t* at = pa + uint64_t(s) * p.step * 2u;
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) lds_copy16(at, oa[i], base + slot * L::kA + i * TH * 16u + wave * 1024u);
+    };
+    // A thread's block: row n0 + tid / 2, half tid & 1 of the step; with TR row
+    // tid / (BN / 32) of the step, block tid % (BN / 32) of the tile's columns.
+    constexpr uint32_t kAcross = BN / 32u;
+    uint4 code;
+    uint32_t byte;
+    auto load_b = [&](uint32_t s) {
+        const uint32_t j = s % p.J;
+        const uint64_t row = TR ? min(j * 64u + tid / kAcross, uint32_t(p.w.rows) - 1u) : min(n0 + tid / 2u, p.N - 1u);
+        const uint64_t blk = row * (4u * p.S) + (TR ? min(n0 / 32u + tid % kAcross, 4u * p.S - 1u) : j * 2u + (tid & 1u));
+        code = reinterpret_cast<const uint4*>(p.w.codes)[blk];
+        byte = p.w.scales[blk];
+    };
+    auto write_b = [&](uint32_t slot) {
+        uint8_t* to = lds + 3u * L::kA + slot * L::kB;
+        const float scale = mx_scale(byte);
+        const uint32_t word[4] = {code.x, code.y, code.z, code.w};
+#pragma unroll
+        for (uint32_t q = 0; q < 4u; ++q) {
+            const uint32_t row = TR ? tid / kAcross : tid / 2u;
+            const uint32_t at = TR ? row * (BN * 2u) + ((tid % kAcross * 2u + q / 2u) ^ (row & 3u)) * 32u + q % 2u * 16u
+                                   : row * 128u + (((tid & 1u) * 4u + q) ^ (row >> 1 & 7u)) * 16u;
+            *reinterpret_cast<bf16x8*>(to + at) = decode8(word[q], scale);
+        }
+    };
+
+    const uint32_t wm = wave / VN * (BM / VM), wn = wave % VN * (BN / VN);
+    f32x16 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    auto compute = [&](uint32_t sa, uint32_t sb) {
+        const uint8_t *la = lds + sa * L::kA, *lb = lds + 3u * L::kA + sb * L::kB;
+#pragma unroll
+        for (uint32_t q = 0; q < 4u; ++q) {   // values 16 q + 8 h .. of the step
+            bf16x8 a[MI], b[NI];
+            const uint32_t at = r * 128u + ((2u * q + h) ^ (r >> 1 & 7u)) * 16u;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const bf16x8*>(la + (wm + 32u * i) * 128u + at);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                if constexpr (TR) {
+                    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+                    const uint32_t i = lane & 15u, row = 16u * q + 8u * h + (i >> 2);
+                    const uint32_t u = ((wn + 32u * j) / 16u + (lane >> 4 & 1u)) ^ (i >> 2);
+                    const uint8_t* from = lb + row * (BN * 2u) + u * 32u + (i & 3u) * 8u;
+                    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)from);
+                    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                        (__attribute__((address_space(3))) bf16x4*)(from + 4u * BN * 2u));
+                    b[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                } else {
+                    b[j] = *reinterpret_cast<const bf16x8*>(lb + (wn + 32u * j) * 128u + at);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+        }
+    };
+
+    // s1 - s0 >= 1; past the end the last step again, unused
+    fetch_a(s0, 0);
+    load_b(s0);
+    wait_vmcnt<0>();
+    write_b(0);
+    fetch_a(min(s0 + 1u, s1 - 1u), 1);
+    load_b(min(s0 + 1u, s1 - 1u));
+    lds_barrier();
+    uint32_t sa = 0, sb = 0;
+    for (uint32_t s = s0; s < s1; ++s) {
+        wait_vmcnt<0>();                         // the next step: its copies have landed
+        write_b(sb ^ 1u);                        // the slots written and copied to are
+        const uint32_t to = sa == 0 ? 2u : sa - 1u;
+        fetch_a(min(s + 2u, s1 - 1u), to);       // the step before's, read out before the
+        load_b(min(s + 2u, s1 - 1u));            // last barrier
+        compute(sa, sb);
+        lds_barrier();
+        sa = sa == 2u ? 0u : sa + 1u;
+        sb ^= 1u;
+    }
+    wait_vmcnt<0>();
+    lds_barrier();
+    ElemT<OT>* o = out + uint64_t(cut) * p.M * ldo;
+    uint8_t* piece = lds + wave * Pc::kBytes;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                Pc::put(piece, r, 8u * e + 4u * h,
+                        f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]});
+            wave_lds_sync();
+            Pc::flush(piece, o, ldo, m0 + wm + 32u * i, n0 + wn + 32u * j, p.M, p.N);
+            wave_lds_sync();
+        }
+}
+
+// out = the sum of the parts, first to last.
+template <int OT>
+__global__ __launch_bounds__(256) void k_mx_join(const float* part, uint32_t parts, uint64_t M, uint32_t N, ElemT<OT>* out,
+                                                 uint64_t ldo) {
+    const uint64_t n = M * N;
+    for (uint64_t i = uint64_t(blockIdx.x) * 256u + threadIdx.x; i < n; i += uint64_t(gridDim.x) * 256u) {
+        float v = part[i];
+        for (uint32_t k = 1; k < parts; ++k) v += part[k * n + i];
+        const uint64_t r = n >> 32 ? i / N : uint32_t(i) / N;
+        out[r * ldo + (i - r * N)] = ElemT<OT>(v);
+    }
+}
+// dx of no rows at all.
+template <int OT>
+__global__ __launch_bounds__(256) void k_mx_zero(uint64_t M, uint32_t N, ElemT<OT>* out, uint64_t ldo) {
+    for (uint64_t i = uint64_t(blockIdx.x) * 256u + threadIdx.x; i < M * N; i += uint64_t(gridDim.x) * 256u)
+        out[i / N * ldo + i % N] = ElemT<OT>(0.0f);
+}
+
+uint32_t blocks_for(uint64_t items) { return uint32_t(std::min<uint64_t>((items + 255u) / 256u, 1u << 20)); }
+
+// How a product of M real rows of J values with N columns runs: tiles of 256
+// or 128, the sum in parts where the tiles leave compute units idle (at least
+// four steps of 64 a part, and no more partial sums than 64 MiB).
+struct RealPlan {
+    uint32_t tile, tm, tn, parts, steps, planes;
+};
+RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
+    RealPlan r;
+    r.planes = dtype == GF_BF16 ? 1u : dtype == GF_F16 ? 2u : 3u;
+    r.steps = uint32_t((J + 63u) / 64u);
+    const uint64_t big = ((M + 255u) / 256u) * ((N + 255u) / 256u);
+    r.tile = big >= 192u ? 256u : 128u;
+    r.tm = uint32_t((M + r.tile - 1u) / r.tile), r.tn = uint32_t((N + r.tile - 1u) / r.tile);
+    const uint64_t tiles = uint64_t(r.tm) * r.tn;
+    uint64_t parts = std::min<uint64_t>(512u / tiles, uint64_t(r.steps) * r.planes / 4u);
+    parts = std::min<uint64_t>(parts, (64u << 20) / (M * N * 4u));
+    r.parts = uint32_t(std::max<uint64_t>(parts, 1u));
+    return r;
+}
+// Whether the real side can be read in place: bfloat16 rows of whole steps,
+// aligned for the copies.
+bool in_place(const MatIn& a, uint64_t J) {
+    return a.dtype == GF_BF16 && J % 64u == 0 && a.ld % 8u == 0 && reinterpret_cast<uintptr_t>(a.p) % 16u == 0 && a.ld < 1u << 22;
+}
+
+template <bool TR>
+hipError_t real_product(const MatIn& a, uint64_t J, const gf_mx_rows& w, uint64_t N, const MatOut& out, void* ws,
+                        hipStream_t st) {
+    const RealPlan pl = real_plan(a.dtype, a.rows, N, J);
+    RealArgs p = {static_cast<const uint16_t*>(a.p), a.ld, 64, pl.planes, uint32_t(a.rows), pl.steps, w, mx_chunks(w.K), uint32_t(N),
+                  pl.tm, pl.tn, pl.parts};
+    uint8_t* at = static_cast<uint8_t*>(ws);
+    if (!in_place(a, J)) {
+        p.a = reinterpret_cast<const uint16_t*>(at), p.lda = 64, p.step = a.rows * 64u;
+        const hipError_t e = by_type(a.dtype, [&](auto dt) {
+            constexpr int DT = decltype(dt)::value;
+            hipLaunchKernelGGL(k_mx_planes<DT>, dim3(blocks_for(a.rows * pl.steps * 8u)), 256, 0, st,
+                               static_cast<const ElemT<DT>*>(a.p), a.rows, uint32_t(J), a.ld, pl.steps,
+                               reinterpret_cast<uint16_t*>(at));
+            return hipGetLastError();
+        });
+        if (e != hipSuccess) return e;
+        at += a.rows * pl.steps * pl.planes * 128u;
+    }
+    auto run = [&](auto ot, void* to, uint64_t ldo) {
+        constexpr int OT = decltype(ot)::value;
+        if (pl.tile == 256u)
+            hipLaunchKernelGGL((k_mx_real<256, 256, 2, 4, OT, TR>), dim3(pl.tm * pl.tn * pl.parts), 512, 0, st, p,
+                               static_cast<ElemT<OT>*>(to), ldo);
+        else
+            hipLaunchKernelGGL((k_mx_real<128, 128, 2, 2, OT, TR>), dim3(pl.tm * pl.tn * pl.parts), 256, 0, st, p,
+                               static_cast<ElemT<OT>*>(to), ldo);
+        return hipGetLastError();
+    };
+    if (pl.parts == 1u) return by_type(out.dtype, [&](auto ot) { return run(ot, out.p, out.ld); });
+    if (const hipError_t e = run(std::integral_constant<int, GF_F32>(), at, N)) return e;
+    return by_type(out.dtype, [&](auto ot) {
+        constexpr int OT = decltype(ot)::value;
+        hipLaunchKernelGGL(k_mx_join<OT>, dim3(blocks_for(a.rows * N)), 256, 0, st, reinterpret_cast<const float*>(at), pl.parts,
+                           a.rows, uint32_t(N), static_cast<ElemT<OT>*>(out.p), out.ld);
+        return hipGetLastError();
+    });
+}
+
+constexpr uint64_t kFew = 16;   // queries that k_mx_few takes
+
+}  // namespace
+
+hipError_t launch_mx_product(const MatIn& x, const gf_mx_rows& w, const MatOut& out, void* ws, hipStream_t st) {
+    if (x.rows > kFew) return real_product<false>(x, w.K, w, w.rows, out, ws, st);
+    const uint32_t S = mx_chunks(w.K);
+    return by_type(x.dtype, [&](auto dt) {
+        return by_type(out.dtype, [&](auto ot) {
+            constexpr int DT = decltype(dt)::value, OT = decltype(ot)::value;
+            auto go = [&](auto nt, auto wk) {
+                constexpr int NT = decltype(nt)::value, WK = decltype(wk)::value;
+                hipLaunchKernelGGL((k_mx_few<DT, NT, WK, OT>), dim3(uint32_t((w.rows + 16u * NT - 1u) / (16u * NT))), 64 * WK, 0,
+                                   st, static_cast<const ElemT<DT>*>(x.p), uint32_t(x.rows), x.ld, w, S,
+                                   static_cast<ElemT<OT>*>(out.p), out.ld);
+                return hipGetLastError();
+            };
+            if (S >= 8) return go(std::integral_constant<int, 2>(), std::integral_constant<int, 8>());
+            return go(std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
+        });
+    });
+}
+
+hipError_t launch_mx_product_grad(const MatIn& dy, const gf_mx_rows& w, const MatOut& dx, void* ws, hipStream_t st) {
+    if (w.rows) return real_product<true>(dy, w.rows, w, w.K, dx, ws, st);
+    return by_type(dx.dtype, [&](auto ot) {
+        constexpr int OT = decltype(ot)::value;
+        hipLaunchKernelGGL(k_mx_zero<OT>, dim3(blocks_for(dy.rows * w.K)), 256, 0, st, dy.rows, w.K,
+                           static_cast<ElemT<OT>*>(dx.p), dx.ld);
+        return hipGetLastError();
+    });
+}
+
+size_t mx_workspace(int32_t kind, int32_t dtype, uint64_t M, uint64_t rows, uint32_t K) {
+    if (kind == 1 || !M || !rows || (kind == 0 && M <= kFew)) return 0;
+    const uint64_t J = kind == 2 ? rows : K, N = kind == 2 ? K : rows;
+    const RealPlan pl = real_plan(dtype, M, N, J);
+    // room for the planes whether or not the real side can be read in place
+    return size_t(pl.steps) * 128u * pl.planes * M + (pl.parts > 1u ? size_t(pl.parts) * M * N * 4u : 0u);
+}
+
+}  // namespace gf

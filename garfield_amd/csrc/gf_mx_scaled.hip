@@ -5,6 +5,8 @@
 // blocks are the instruction's, so codes and scales go to it as they lie in
 // memory.  w's rows are the first operand, so that a lane ends with four
 // consecutive columns of the result.
+#include <algorithm>
+
 #include "gf_mx_device.h"
 
 namespace gf {
@@ -32,7 +34,7 @@ template <int MT, int NT, int WN, int WK, int OT>
 __global__ __launch_bounds__(64 * WN * WK) void k_mx_direct(gf_mx_rows x, gf_mx_rows w, uint32_t S, uint32_t tm,
                                                             uint32_t tn, ElemT<OT>* out, uint64_t ldo) {
     constexpr uint32_t kJoin = WK > 1 ? WK * 64u * MT * NT * 16u : 0u;
-    constexpr uint32_t kPieces = MT >= 2 && NT == 4 ? WN * Piece<OT>::kBytes : 0u;
+    constexpr uint32_t kPieces = MT >= 2 && NT == 4 ? WN * Piece<OT, 64>::kBytes : 0u;
     __shared__ __align__(16) uint8_t lds[kJoin > kPieces ? kJoin : kPieces ? kPieces : 16u];
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
     const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
@@ -94,16 +96,16 @@ __global__ __launch_bounds__(64 * WN * WK) void k_mx_direct(gf_mx_rows x, gf_mx_
                 for (uint32_t k = 1; k < WK; ++k) acc[i][j] += part[(k * MT * NT + i * NT + j) * 64u + lane];
     }
     if constexpr (kPieces != 0) {
-        uint8_t* piece = lds + wn * Piece<OT>::kBytes;
+        uint8_t* piece = lds + wn * Piece<OT, 64>::kBytes;
         if (WK > 1) wave_lds_sync();   // WN is 1 then: the parts were read by this wave alone
 #pragma unroll
         for (int i = 0; i < MT; i += 2) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) Piece<OT>::put(piece, 16u * h + r, 16u * j + 4u * g, acc[i + h][j]);
+                for (int j = 0; j < NT; ++j) Piece<OT, 64>::put(piece, 16u * h + r, 16u * j + 4u * g, acc[i + h][j]);
             wave_lds_sync();
-            Piece<OT>::flush(piece, out, ldo, m0 + 16u * i, n0, M, N);
+            Piece<OT, 64>::flush(piece, out, ldo, m0 + 16u * i, n0, M, N);
             wave_lds_sync();
         }
     } else {
@@ -119,125 +121,181 @@ __global__ __launch_bounds__(64 * WN * WK) void k_mx_direct(gf_mx_rows x, gf_mx_
 }
 
 // ---- operands through LDS --------------------------------------------------
-// A block has a tile of BM queries x BN rows, its VM x VN waves equal parts of
-// it, and takes 256 values (8 blocks, 128 bytes of codes) of each row a step.
-// While one half of LDS is computed on, loads straight to LDS fill the other.
-// Of a row's 8 blocks, lane group h (of two) takes blocks 4 h + s in step s,
-// on both sides alike: its four scale bytes are then one word.  The 16-byte
-// chunk c of row r lies at place c ^ (r & 7) of the row, so that eight
-// consecutive rows read one chunk from eight different places.
+// A block takes tiles of BM queries x BN rows one after another, its VM x VN
+// waves equal parts of one, and a chunk of 128 values (4 blocks) of each row a
+// step.  Steps, of all its tiles in one sequence, go through kSlots slots of
+// LDS, filled by copies that pass no register: while a step is computed on,
+// the next three are on the way.  A step has two parts; a part's operands are
+// read from LDS while the part before it is multiplied, across steps too.
+// Branches stand before a step's products only: the compiler moves matrix
+// instructions down past a branch, and a barrier would then find the matrix
+// cores idle.
+// Of a row's 4 blocks lane group h (of two) takes blocks 2 h and 2 h + 1, on
+// both sides alike: its scale bytes are then the low ones of a shifted word.
+// The 16-byte block c of row r lies at place c ^ (r / 4 & 3) of the row: four
+// rows of 64 bytes cover the banks, so of 16 rows the four that share banks
+// have a block in four different places.
+// Scales come 16 bytes a row, for four steps at once: a line is asked for once
+// for four steps.  A tile's last group ends with the row (S >= 4), so that no
+// read passes the end.  Groups are of four steps or, at the end of a tile,
+// fewer, but never twice in a row: the four steps under way lie in three groups
+// at most.
+constexpr uint32_t kSlots = 4, kGroups = 3;
+
+template <int BM, int BN, int OT>
+struct TileLds {
+    static constexpr uint32_t kRows = BM + BN, kSlot = kRows * 64u, kGroup = kRows * 16u;
+    static constexpr uint32_t kBytes = kSlots * kSlot + kGroups * kGroup;
+    static constexpr uint32_t kCols = OT == GF_F32 ? 16u : 32u;   // of a piece: 64-byte rows
+    using P = Piece<OT, kCols>;
+};
+
 template <int BM, int BN, int VM, int VN, int OT>
 __global__ __launch_bounds__(64 * VM * VN) void k_mx_tile(gf_mx_rows x, gf_mx_rows w, uint32_t S, uint32_t tm,
                                                           uint32_t tn, ElemT<OT>* out, uint64_t ldo) {
-    constexpr uint32_t TH = 64u * VM * VN, kRows = BM + BN, kCodes = kRows * 128u, kHalf = kCodes + kRows * 8u;
-    constexpr uint32_t kPer = kRows * 8u / TH;    // 16-byte loads a thread and step
-    constexpr uint32_t kPerS = kRows * 2u / TH;   // scale words a thread and step
+    using L = TileLds<BM, BN, OT>;
+    using P = typename L::P;
+    constexpr uint32_t TH = 64u * VM * VN, kRows = L::kRows, kSlot = L::kSlot;
+    constexpr uint32_t kPer = kRows * 4u / TH, kPerS = kRows / TH;   // copies a thread and step, and group
     constexpr int MI = BM / VM / 32, NI = BN / VN / 32;
-    constexpr uint32_t kPieces = VM * VN * Piece<OT>::kBytes;
-    static_assert(NI == 2 && kRows * 2u % TH == 0, "");
-    __shared__ __align__(16) uint8_t lds[2u * kHalf > kPieces ? 2u * kHalf : kPieces];
+    static_assert(kRows % TH == 0 && TH % 64u == 0 && VM * VN * P::kBytes <= kSlot, "");
+    __shared__ __align__(16) uint8_t lds[L::kBytes];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, r = lane & 31u, h = lane >> 5;
     const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(tid >> 6)));
-    const uint32_t M = uint32_t(x.rows), N = uint32_t(w.rows);
-    uint32_t bm, bn;
-    tile_of(xcd_run(blockIdx.x, tm * tn), tm, tn, 4u, bm, bn);
-    const uint32_t m0 = bm * BM, n0 = bn * BN;
-
-    // LDS row i of a half: query m0 + i, or row n0 + i - BM of w; beyond the
-    // ends the last row again (its sums are not stored).
-    const uint8_t *pc[kPer], *ps[kPerS];
-    auto row_at = [&](uint32_t i, uint32_t width, const uint8_t* cx, const uint8_t* cw) {
-        return i < BM ? cx + uint64_t(min(m0 + i, M - 1u)) * S * width : cw + uint64_t(min(n0 + i - BM, N - 1u)) * S * width;
+    const uint32_t M = uint32_t(x.rows), N = uint32_t(w.rows), tiles = tm * tn;
+    const uint32_t base = lds_addr(lds);
+    auto corner = [&](uint32_t t, uint32_t& m0, uint32_t& n0) {
+        tile_of(xcd_run(t, tiles), tm, tn, 4u, m0, n0);
+        m0 *= BM, n0 *= BN;
     };
-    const uint32_t chunk = (tid & 7u) ^ (tid >> 3 & 7u);
-#pragma unroll
-    for (uint32_t i = 0; i < kPer; ++i)
-        pc[i] = row_at(i * (TH / 8u) + tid / 8u, 64u, x.codes, w.codes) + chunk * 16u;
-#pragma unroll
-    for (uint32_t i = 0; i < kPerS; ++i)
-        ps[i] = row_at(i * (TH / 2u) + tid / 2u, 4u, x.scales, w.scales) + (tid & 1u) * 4u;
 
-    auto fetch = [&](uint32_t step, uint32_t half) {
-        uint8_t* base = lds + half * kHalf;
-        const bool whole = 2u * step + 2u <= S;
-        if (whole || chunk < 4u) {
+    // The copies' cursor: tile ft, step fs, scale group fg.  LDS row i of a
+    // slot: query m0 + i, or row n0 + i - BM of w; beyond the ends the last row
+    // again (its sums are not stored).
+    uint32_t ft = blockIdx.x, fs = 0, fg = 0, oc[kPer], os[kPerS];
+    const uint8_t *xc, *wc, *xs, *ws;   // of the tile's first row
+    auto aim = [&]() {
+        uint32_t m0, n0;
+        corner(ft, m0, n0);
+        xc = x.codes + uint64_t(m0) * S * 64u, wc = w.codes + uint64_t(n0) * S * 64u;
+        xs = x.scales + uint64_t(m0) * S * 4u, ws = w.scales + uint64_t(n0) * S * 4u;
+        auto row = [&](uint32_t i) { return i < BM ? min(i, M - 1u - m0) : min(i - BM, N - 1u - n0); };
 #pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i)
-                __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void*)(pc[i] + uint64_t(step) * 128u),
-                    (__attribute__((address_space(3))) void*)(base + i * TH * 16u + wave * 1024u), 16, 0, 0);
-        } else {   // an odd last chunk of 128: the other half of the step is zeros
+        for (uint32_t i = 0; i < kPer; ++i) oc[i] = row(i * (TH / 4u) + tid / 4u) * (S * 64u) + ((tid & 3u) ^ (tid >> 4 & 3u)) * 16u;
 #pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i) *reinterpret_cast<uint4*>(base + (i * TH + tid) * 16u) = make_uint4(0, 0, 0, 0);
-        }
-        if (whole || !(tid & 1u)) {
+        for (uint32_t i = 0; i < kPerS; ++i) os[i] = row(i * TH + tid) * (S * 4u);
+    };
+    // Past the last tile the copies go on from the last one's rows, unused, so
+    // that as many are always under way.
+    auto fetch = [&](uint32_t slot) {
+        if ((fs & 3u) == 0) {
+            const uint32_t at = base + kSlots * kSlot + fg * L::kGroup;
+            const uint32_t from = min(fs, S - 4u) * 4u;
 #pragma unroll
             for (uint32_t i = 0; i < kPerS; ++i)
-                __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void*)(ps[i] + uint64_t(step) * 8u),
-                    (__attribute__((address_space(3))) void*)(base + kCodes + i * TH * 4u + wave * 256u), 4, 0, 0);
-        } else {
+                lds_copy16((i * TH + wave * 64u < BM ? xs : ws) + from, os[i], at + i * TH * 16u + wave * 1024u);
+            fg = fg + 1u == kGroups ? 0u : fg + 1u;
+        }
+        const uint32_t at = base + slot * kSlot;
 #pragma unroll
-            for (uint32_t i = 0; i < kPerS; ++i) *reinterpret_cast<uint32_t*>(base + kCodes + (i * TH + tid) * 4u) = 0u;
+        for (uint32_t i = 0; i < kPer; ++i)
+            lds_copy16((i * (TH / 4u) < BM ? xc : wc) + uint64_t(fs) * 64u, oc[i], at + i * TH * 16u + wave * 1024u);
+        if (++fs == S) {
+            fs = 0;
+            ft += gridDim.x;
+            if (ft < tiles) aim();
         }
     };
 
     const uint32_t wm = wave / VN * (BM / VM), wn = wave % VN * (BN / VN);
     f32x16 acc[MI][NI];
+    uint4 a[2][MI], b[2][NI];
+    uint32_t sa[2][MI], sb[2][NI];
+    uint32_t rs = 0, rg = kGroups - 1u;   // the step whose first part is read next, and its group's place
+    // Part 0 or 1 of the step in `slot`.
+    auto read = [&](uint32_t slot, auto part) {
+        constexpr int B = decltype(part)::value;
+        const uint8_t* p = lds + slot * kSlot;
+        const uint32_t at = r * 64u + ((2u * h + B) ^ (r >> 2 & 3u)) * 16u;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < MI; ++i) a[B][i] = *reinterpret_cast<const uint4*>(p + (wm + 32u * i) * 64u + at);
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
+        for (int j = 0; j < NI; ++j) b[B][j] = *reinterpret_cast<const uint4*>(p + (BM + wn + 32u * j) * 64u + at);
+        if (B == 0) {
+            if ((rs & 3u) == 0) rg = rg + 1u == kGroups ? 0u : rg + 1u;
+            const uint32_t q = (rs | 3u) < S ? rs & 3u : rs - (S - 4u);   // the step's word in its group
+            const uint8_t* g = lds + kSlots * kSlot + rg * L::kGroup + q * 4u;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-
-    auto part = [&](const uint8_t* base, const uint32_t* sa, const uint32_t* sb, auto byte) {
-        constexpr int B = decltype(byte)::value;
-        const uint32_t at = r * 128u + ((4u * h + B) ^ (r & 7u)) * 16u;
-        uint4 a[MI], b[NI];
+            for (int i = 0; i < MI; ++i) sa[0][i] = *reinterpret_cast<const uint32_t*>(g + (wm + 32u * i + r) * 16u) >> (16u * h);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const uint4*>(base + (wm + 32u * i) * 128u + at);
+            for (int j = 0; j < NI; ++j) sb[0][j] = *reinterpret_cast<const uint32_t*>(g + (BM + wn + 32u * j + r) * 16u) >> (16u * h);
+            rs = rs + 1u == S ? 0u : rs + 1u;
+        } else {
 #pragma unroll
-        for (int j = 0; j < NI; ++j) b[j] = *reinterpret_cast<const uint4*>(base + (BM + wn + 32u * j) * 128u + at);
+            for (int i = 0; i < MI; ++i) sa[1][i] = sa[0][i];
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = mfma32<B>(b[j], sb[j], a[i], sa[i], acc[i][j]);
+            for (int j = 0; j < NI; ++j) sb[1][j] = sb[0][j];
+        }
     };
-
-    const uint32_t steps = (S + 1u) / 2u;
-    fetch(0, 0);
-    for (uint32_t s = 0; s < steps; ++s) {
-        __builtin_amdgcn_s_waitcnt(0x0F70);   // this wave's loads to LDS have landed
-        __syncthreads();                      // and the others'; the other half has been read
-        if (s + 1u < steps) fetch(s + 1u, (s + 1u) & 1u);
-        const uint8_t* base = lds + (s & 1u) * kHalf;
-        uint32_t sa[MI], sb[NI];
+    auto multiply = [&](auto part) {
+        constexpr int B = decltype(part)::value;
+        sched_fence();
 #pragma unroll
         for (int i = 0; i < MI; ++i)
-            sa[i] = *reinterpret_cast<const uint32_t*>(base + kCodes + ((wm + 32u * i + r) * 2u + h) * 4u);
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
-            sb[j] = *reinterpret_cast<const uint32_t*>(base + kCodes + ((BM + wn + 32u * j + r) * 2u + h) * 4u);
-        part(base, sa, sb, std::integral_constant<int, 0>());
-        part(base, sa, sb, std::integral_constant<int, 1>());
-        part(base, sa, sb, std::integral_constant<int, 2>());
-        part(base, sa, sb, std::integral_constant<int, 3>());
+            for (int j = 0; j < NI; ++j) acc[i][j] = mfma32<B>(b[B][j], sb[B][j], a[B][i], sa[B][i], acc[i][j]);
+        sched_fence();
+    };
+    const std::integral_constant<int, 0> first;
+    const std::integral_constant<int, 1> second;
+
+    aim();
+    fetch(0);
+    fetch(1);
+    fetch(2);
+    wait_vmcnt<2u * kPer>();   // this wave's part of the first step has landed,
+    lds_barrier();             // and the others'
+    read(0, first);
+    uint32_t slot = 0;
+    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+        for (uint32_t s = 0; s < S; ++s) {
+            fetch((slot + 3u) % kSlots);   // the step before's slot, read out before the last barrier
+            read(slot, second);
+            multiply(first);
+            wait_vmcnt<2u * kPer>();       // the next step's copies
+            lds_barrier();
+            slot = (slot + 1u) % kSlots;
+            read(slot, first);             // after the last step of all: bytes that nothing uses
+            multiply(second);
+        }
+        uint32_t m0, n0;
+        corner(t, m0, n0);
+        // the last step's slot is read out: the pieces' until the next copies
+        uint8_t* piece = lds + (slot + 3u) % kSlots * kSlot + wave * P::kBytes;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int q = 0; q < int(32u / L::kCols); ++q) {
+#pragma unroll
+                    for (int e = 0; e < int(L::kCols / 8u); ++e) {
+                        const int k = 4 * (e + q * int(L::kCols / 8u));
+                        P::put(piece, r, 8u * e + 4u * h, f32x4{acc[i][j][k], acc[i][j][k + 1], acc[i][j][k + 2], acc[i][j][k + 3]});
+                    }
+                    wave_lds_sync();
+                    P::flush(piece, out, ldo, m0 + wm + 32u * i, n0 + wn + 32u * j + L::kCols * q, M, N);
+                    wave_lds_sync();
+                }
+        lds_barrier();   // every wave has read its last piece
     }
-    __syncthreads();
-    uint8_t* piece = lds + wave * Piece<OT>::kBytes;
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-#pragma unroll
-        for (int j = 0; j < NI; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                Piece<OT>::put(piece, r, 32u * j + 8u * e + 4u * h,
-                               f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]});
-        wave_lds_sync();
-        Piece<OT>::flush(piece, out, ldo, m0 + wm + 32u * i, n0 + wn, M, N);
-        wave_lds_sync();
-    }
+    wait_vmcnt<0>();   // no copy outlives the block
 }
 
 template <int MT, int NT, int WN, int WK>
@@ -256,7 +314,9 @@ hipError_t tile(const gf_mx_rows& x, const gf_mx_rows& w, const MatOut& out, hip
     const uint32_t tm = uint32_t((x.rows + BM - 1u) / BM), tn = uint32_t((w.rows + BN - 1u) / BN);
     return by_type(out.dtype, [&](auto ot) {
         constexpr int OT = decltype(ot)::value;
-        hipLaunchKernelGGL((k_mx_tile<BM, BN, VM, VN, OT>), dim3(tm * tn), 64 * VM * VN, 0, st, x, w, mx_chunks(w.K), tm,
+        // as many blocks as the chip's LDS holds at once
+        const uint32_t blocks = std::min(tm * tn, compute_units() * (160u * 1024u / TileLds<BM, BN, OT>::kBytes));
+        hipLaunchKernelGGL((k_mx_tile<BM, BN, VM, VN, OT>), dim3(blocks), 64 * VM * VN, 0, st, x, w, mx_chunks(w.K), tm,
                            tn, static_cast<ElemT<OT>*>(out.p), out.ld);
         return hipGetLastError();
     });
@@ -270,8 +330,8 @@ hipError_t launch_mx_product_mx(const gf_mx_rows& x, const gf_mx_rows& w, const 
     if (M <= 16) return S >= 8 ? direct<1, 1, 1, 8>(x, w, out, st) : direct<1, 1, 1, 1>(x, w, out, st);
     if (S >= 4) {
         const uint64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
-        if (big >= 192) return tile<256, 256, 2, 4>(x, w, out, st);
-        if (mid >= 128) return tile<128, 128, 2, 2>(x, w, out, st);
+        if (big >= 192 && S < 1u << 18) return tile<256, 256, 2, 4>(x, w, out, st);
+        if (mid >= 128 && S < 1u << 18) return tile<128, 128, 2, 2>(x, w, out, st);
         return direct<4, 4, 1, 4>(x, w, out, st);
     }
     return direct<4, 4, 4, 1>(x, w, out, st);
