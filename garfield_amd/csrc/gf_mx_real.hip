@@ -44,12 +44,13 @@ __device__ __forceinline__ void split8(const float* v, uint4* plane) {
     for (int p = 0; p < P; ++p) plane[p] = make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
 }
 
-// Eight elements of a row from k on, zeros from K on, as planes.
-template <int DT>
+// Eight elements of a row from k on, zeros from K on (WHOLE: all below K), as
+// planes.
+template <int DT, bool WHOLE = false>
 __device__ __forceinline__ void load_planes(const ElemT<DT>* row, uint32_t k, uint32_t K, uint4* plane) {
     constexpr int P = kPlanes<DT>;
     ElemT<DT> e[8];
-    if (k + 8u <= K) {
+    if (WHOLE || k + 8u <= K) {
 #pragma unroll
         for (uint32_t i = 0; i < sizeof(e) / 16u; ++i) {
             const uint4 q = load16(reinterpret_cast<const uint8_t*>(row + k) + i * 16u);
@@ -104,7 +105,8 @@ __global__ __launch_bounds__(256) void k_mx_planes(const ElemT<DT>* x, uint64_t 
 
 // ---- few queries -----------------------------------------------------------
 // Up to 16 queries: w is read once, straight to registers, and nothing else
-// counts.  A wave has 16 NT rows of w; the block's WK waves share them, each
+// counts: one query against 16384 rows of 4096 (37 MB) takes 9.8 us, 3.6 TB/s,
+// where loads of the same shape alone take 8.4.  A wave has 16 NT rows of w; the block's WK waves share them, each
 // with its part of K, joined in order through LDS.  Lane group g of four holds
 // block g of a chunk's four, 16 bytes; the values 8 q .. 8 q + 7 of the four
 // blocks go through one instruction, on both sides alike.
@@ -123,31 +125,19 @@ __global__ __launch_bounds__(64 * WK) void k_mx_few(const ElemT<DT>* x, uint32_t
     for (int j = 0; j < NT; ++j) {   // rows beyond the end repeat the last one; their sums are not stored
         const uint64_t row = min(n0 + 16u * j + r, N - 1u);
         wc[j] = w.codes + row * S * 64u + g * 16u;
-        ws[j] = w.scales + row * S * 4u + g;
+        ws[j] = w.scales + row * S * 4u;
     }
-    const ElemT<DT>* xr = x + uint64_t(min(r, M - 1u)) * ldx;
-    const uint32_t s1 = uint32_t(uint64_t(S) * (wk + 1u) / WK);
-#pragma unroll 2
-    for (uint32_t s = uint32_t(uint64_t(S) * wk / WK); s < s1; ++s) {
+    const ElemT<DT>* xr = x + uint64_t(min(r, M - 1u)) * ldx;   // lanes without a query: the last again, not stored
+    // Chunk s, byte[j] the scale byte of its block.
+    auto chunk = [&](uint32_t s, const uint32_t* byte, auto whole) {
         uint4 c[NT], a[4][P];
-        uint32_t sc[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) c[j] = *reinterpret_cast<const uint4*>(wc[j] + uint64_t(s) * 64u);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) load_planes<DT, decltype(whole)::value>(xr, s * 128u + g * 32u + q * 8u, K, a[q]);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            c[j] = *reinterpret_cast<const uint4*>(wc[j] + uint64_t(s) * 64u);
-            sc[j] = ws[j][uint64_t(s) * 4u];
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (r < M) {
-                load_planes<DT>(xr, s * 128u + g * 32u + q * 8u, K, a[q]);
-            } else {
-#pragma unroll
-                for (int p = 0; p < P; ++p) a[q][p] = make_uint4(0, 0, 0, 0);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const float scale = mx_scale(sc[j]);
+            const float scale = mx_scale(byte[j]);
             const uint32_t word[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -157,6 +147,31 @@ __global__ __launch_bounds__(64 * WK) void k_mx_few(const ElemT<DT>* x, uint32_t
                     acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, as_bf16x8(a[q][p]), acc[j], 0, 0, 0);
             }
         }
+    };
+    // Four whole chunks at a time: no branch stands between their loads, and a
+    // row's scales come in one.  Then what is left, the last chunk perhaps cut.
+    const uint32_t s1 = uint32_t(uint64_t(S) * (wk + 1u) / WK), cut = min(s1, K / 128u);
+    uint32_t s = uint32_t(uint64_t(S) * wk / WK);
+    for (; s + 4u <= cut; s += 4u) {
+        uint4 sc[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sc[j] = load16(ws[j] + uint64_t(s) * 4u);
+#pragma unroll
+        for (uint32_t u = 0; u < 4u; ++u) {
+            uint32_t byte[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const uint32_t word[4] = {sc[j].x, sc[j].y, sc[j].z, sc[j].w};
+                byte[j] = word[u] >> (8u * g) & 255u;
+            }
+            chunk(s + u, byte, std::true_type());
+        }
+    }
+    for (; s < s1; ++s) {
+        uint32_t byte[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) byte[j] = ws[j][uint64_t(s) * 4u + g];
+        chunk(s, byte, std::false_type());
     }
     if (WK > 1) {
 #pragma unroll
@@ -351,6 +366,7 @@ __global__ __launch_bounds__(256) void k_mx_join(const float* part, uint32_t par
     const uint64_t n = M * N;
     for (uint64_t i = uint64_t(blockIdx.x) * 256u + threadIdx.x; i < n; i += uint64_t(gridDim.x) * 256u) {
         float v = part[i];
+#pragma unroll 8
         for (uint32_t k = 1; k < parts; ++k) v += part[k * n + i];
         const uint64_t r = n >> 32 ? i / N : uint32_t(i) / N;
         out[r * ldo + (i - r * N)] = ElemT<OT>(v);
@@ -367,7 +383,8 @@ uint32_t blocks_for(uint64_t items) { return uint32_t(std::min<uint64_t>((items 
 
 // How a product of M real rows of J values with N columns runs: tiles of 256
 // or 128, the sum in parts where the tiles leave compute units idle (at least
-// four steps of 64 a part, and no more partial sums than 64 MiB).
+// four steps of 64 a part, one part a compute unit, and no more partial sums
+// than 64 MiB).
 struct RealPlan {
     uint32_t tile, tm, tn, parts, steps, planes;
 };
@@ -379,7 +396,7 @@ RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
     r.tile = big >= 192u ? 256u : 128u;
     r.tm = uint32_t((M + r.tile - 1u) / r.tile), r.tn = uint32_t((N + r.tile - 1u) / r.tile);
     const uint64_t tiles = uint64_t(r.tm) * r.tn;
-    uint64_t parts = std::min<uint64_t>(512u / tiles, uint64_t(r.steps) * r.planes / 4u);
+    uint64_t parts = std::min<uint64_t>(256u / tiles, uint64_t(r.steps) * r.planes / 4u);
     parts = std::min<uint64_t>(parts, (64u << 20) / (M * N * 4u));
     r.parts = uint32_t(std::max<uint64_t>(parts, 1u));
     return r;
@@ -446,7 +463,14 @@ hipError_t launch_mx_product(const MatIn& x, const gf_mx_rows& w, const MatOut& 
                                    static_cast<ElemT<OT>*>(out.p), out.ld);
                 return hipGetLastError();
             };
-            if (S >= 8) return go(std::integral_constant<int, 2>(), std::integral_constant<int, 8>());
+            // Many queries share each decoded block, few are bound by the loads of
+            // codes, and few rows leave compute units idle.  Rows of 4096, 16384
+            // of them: 16 queries 13.7 us by <4, 8> against 15.2 by <2, 4>, one
+            // query 12.0 against 9.8; one query, 4096 rows of 1024: 4.3 us by <2, 4>
+            // against 3.3 by <1, 8>.
+            if (S >= 8 && x.rows > 4) return go(std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
+            if (S >= 8 && w.rows >= 8192) return go(std::integral_constant<int, 2>(), std::integral_constant<int, 4>());
+            if (S >= 8) return go(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
             return go(std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
         });
     });

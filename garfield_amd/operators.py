@@ -19,19 +19,21 @@ from . import _lib
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORES = {"max": 0, "top2": 1}
-_types = None
+torch = None        # imported by the first call: the rest of the package does without
+_types = {}
 
 
-def _torch():
-    import torch
+def _need_torch():
+    global torch
+    if torch is None:
+        import torch as t
+        _types.update({t.float32: 0, t.float16: 1, t.bfloat16: 2})
+        torch = t
     return torch
 
 
 def _type(dtype, what):
-    global _types
-    if _types is None:
-        t = _torch()
-        _types = {t.float32: 0, t.float16: 1, t.bfloat16: 2}
+    _need_torch()
     code = _types.get(dtype)
     if code is None:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, got {dtype}")
@@ -40,41 +42,39 @@ def _type(dtype, what):
 
 def _matrix(x, what):
     """x as the library reads it: (type, rows, columns, row distance)."""
-    if not isinstance(x, _torch().Tensor) or x.ndim != 2:
+    if not isinstance(x, _need_torch().Tensor) or x.ndim != 2:
         raise ValueError(f"{what} must be a matrix (a 2-d tensor)")
     if not x.is_cuda:
         raise ValueError(f"{what} must be on the GPU")
     n, d = x.shape
-    if d > 1 and x.stride(1) != 1:
+    ld, one = x.stride()
+    if one != 1 and d > 1:
         raise ValueError(f"{what}'s last dimension must be contiguous")
-    ld = x.stride(0) if n > 1 else d
-    if ld < d:
+    if n < 2:
+        ld = d
+    elif ld < d:
         raise ValueError(f"{what}'s rows overlap")
     return _type(x.dtype, what), n, d, ld
 
 
-def _vector(x, n, dtype, device, what):
+def _vector(x, shape, dtype, device, what):
     if x is None:
         return None
-    if x.shape != n or x.dtype != dtype or x.device != device or not x.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous {tuple(n)} {dtype} tensor on {device}")
+    if x.shape != shape or x.dtype != dtype or x.device != device or not x.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {tuple(shape)} {dtype} tensor on {device}")
     return x.data_ptr()
 
 
-class _On:
-    """The device and stream of a call's tensors."""
-
-    def __init__(self, device):
-        cuda = _torch().cuda
-        self.stream = cuda.current_stream(device).cuda_stream
-        self.guard = cuda.device(device) if cuda.current_device() != device.index else None
-
-    def call(self, fn, *args):
-        if self.guard is None:
-            _lib._check(fn(*args, self.stream))
-        else:
-            with self.guard:
-                _lib._check(fn(*args, self.stream))
+def _call(device, fn, *args):
+    """fn on the current stream of the tensors' device."""
+    i = device.index
+    if torch._C._cuda_getDevice() == i:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if status:
+        _lib._check(status)
 
 
 class MXRows:
@@ -82,7 +82,7 @@ class MXRows:
     S = ceil(K / 128); the layout is gf_mx_rows'."""
 
     def __init__(self, codes, scales, K):
-        torch = _torch()
+        _need_torch()
         S = -(-int(K) // 128)
         if K < 1:
             raise ValueError("K must be at least 1")
@@ -93,12 +93,12 @@ class MXRows:
                 raise ValueError(f"{what} must be a contiguous (rows, {width}) uint8 tensor on the GPU")
             if t.data_ptr() % align:
                 raise ValueError(f"{what} must be aligned to {align} bytes")
-        self.codes, self.scales, self.K = codes, scales, int(K)
-        self._struct = _lib.MXRowsStruct(codes.data_ptr(), scales.data_ptr(), codes.shape[0], self.K)
+        self._set(codes, scales, int(K))
 
-    @property
-    def rows(self):
-        return self.codes.shape[0]
+    def _set(self, codes, scales, K):
+        self.codes, self.scales, self.K, self.rows = codes, scales, K, codes.shape[0]
+        self._struct = _lib.MXRowsStruct(codes.data_ptr(), scales.data_ptr(), self.rows, K)
+        return self
 
     @property
     def device(self):
@@ -113,26 +113,26 @@ class MXRows:
 
 def mx_quantise(x):
     """The rows of x (n, K) at four bits (gf_mx_quantise)."""
-    torch = _torch()
     t, n, K, ld = _matrix(x, "x")
     if K < 1:
         raise ValueError("x must have at least one column")
     S = -(-K // 128)
-    codes = torch.empty((n, 64 * S), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((n, 4 * S), dtype=torch.uint8, device=x.device)
-    _On(x.device).call(_lib.load().gf_mx_quantise, x.data_ptr(), t, n, K, ld, codes.data_ptr(), scales.data_ptr())
-    return MXRows(codes, scales, K)
+    dev = x.device
+    codes = torch.empty((n, 64 * S), dtype=torch.uint8, device=dev)
+    scales = torch.empty((n, 4 * S), dtype=torch.uint8, device=dev)
+    _call(dev, _lib.load().gf_mx_quantise, x.data_ptr(), t, n, K, ld, codes.data_ptr(), scales.data_ptr())
+    return MXRows.__new__(MXRows)._set(codes, scales, K)
 
 
 def mx_dequantise(w, dtype=None):
     """The values that w's rows stand for, (rows, K), float32 by default."""
-    torch = _torch()
+    _need_torch()
     if not isinstance(w, MXRows):
         raise ValueError("w must be MXRows")
     dtype = dtype or torch.float32
     t = _type(dtype, "dtype")
     out = torch.empty((w.rows, w.K), dtype=dtype, device=w.device)
-    _On(w.device).call(_lib.load().gf_mx_dequantise, C.byref(w._struct), t, out.data_ptr(), w.K)
+    _call(w.device, _lib.load().gf_mx_dequantise, C.byref(w._struct), t, out.data_ptr(), w.K)
     return out
 
 
@@ -141,12 +141,10 @@ def _workspace(kind, t, M, w):
     _lib._check(_lib.load().gf_mx_product_workspace(kind, t, M, w.rows, w.K, C.byref(n)))
     if not n.value:
         return None, 0
-    torch = _torch()
     return torch.empty(n.value, dtype=torch.uint8, device=w.device), n.value
 
 
 def _product(x, w, dtype):
-    torch = _torch()
     if not isinstance(w, MXRows):
         raise ValueError("w must be MXRows")
     lib = _lib.load()
@@ -156,9 +154,9 @@ def _product(x, w, dtype):
         dtype = dtype or torch.float32
         to = _type(dtype, "dtype")
         out = torch.empty((x.rows, w.rows), dtype=dtype, device=w.device)
-        ws, nws = _workspace(1, 0, x.rows, w)
-        _On(w.device).call(lib.gf_mx_product_mx, C.byref(x._struct), C.byref(w._struct), to, out.data_ptr(), w.rows,
-                           ws.data_ptr() if nws else None, nws)
+        # this product takes no workspace
+        _call(w.device, lib.gf_mx_product_mx, C.byref(x._struct), C.byref(w._struct), to, out.data_ptr(), w.rows,
+              None, 0)
         return out
     t, M, K, ld = _matrix(x, "x")
     if K != w.K or x.device != w.device:
@@ -167,15 +165,14 @@ def _product(x, w, dtype):
     to = _type(dtype, "dtype")
     out = torch.empty((M, w.rows), dtype=dtype, device=w.device)
     ws, nws = _workspace(0, t, M, w)
-    _On(w.device).call(lib.gf_mx_product, x.data_ptr(), t, M, ld, C.byref(w._struct), to, out.data_ptr(), w.rows,
-                       ws.data_ptr() if nws else None, nws)
+    _call(w.device, lib.gf_mx_product, x.data_ptr(), t, M, ld, C.byref(w._struct), to, out.data_ptr(), w.rows,
+          ws.data_ptr() if nws else None, nws)
     return out
 
 
 def mx_product_grad(dy, w, dtype=None):
     """The gradient of mx_product(x, w) with respect to x, (M, K), from dy
     (M, rows); dy's type by default (gf_mx_product_grad)."""
-    torch = _torch()
     if not isinstance(w, MXRows):
         raise ValueError("w must be MXRows")
     t, M, N, ld = _matrix(dy, "dy")
@@ -185,8 +182,8 @@ def mx_product_grad(dy, w, dtype=None):
     to = _type(dtype, "dtype")
     dx = torch.empty((M, w.K), dtype=dtype, device=w.device)
     ws, nws = _workspace(2, t, M, w)
-    _On(w.device).call(_lib.load().gf_mx_product_grad, dy.data_ptr(), t, M, ld, C.byref(w._struct), to,
-                       dx.data_ptr(), w.K, ws.data_ptr() if nws else None, nws)
+    _call(w.device, _lib.load().gf_mx_product_grad, dy.data_ptr(), t, M, ld, C.byref(w._struct), to,
+          dx.data_ptr(), w.K, ws.data_ptr() if nws else None, nws)
     return dx
 
 
@@ -197,8 +194,6 @@ def _autograd():
     """The autograd nodes, made at the first call that needs one."""
     global _functions
     if _functions is None:
-        torch = _torch()
-
         class Product(torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, w, dtype):
@@ -235,7 +230,7 @@ def mx_product(x, w, dtype=None):
     """Scores (M, rows) of x against w's rows: x a matrix (M, K), whose values
     enter unrounded, or MXRows.  dtype: the result's type (by default x's, or
     float32 for MXRows).  Differentiable with respect to a matrix x."""
-    if not isinstance(x, MXRows) and isinstance(x, _torch().Tensor) and x.requires_grad and _torch().is_grad_enabled():
+    if isinstance(x, _need_torch().Tensor) and x.requires_grad and torch.is_grad_enabled():
         return _autograd()[0].apply(x, w, dtype)
     return _product(x, w, dtype)
 
@@ -262,7 +257,6 @@ def _choice(table, key, what):
 
 
 def _route(logits, k, bias, groups, keep_groups, group_score, score, renormalise, scale):
-    torch = _torch()
     t, T, E, ld = _matrix(logits, "logits")
     opts = _lib.RouteOpts(int(k), _choice(_SCORES, score, "score"), int(groups), int(keep_groups),
                           _choice(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalise)), float(scale))
@@ -271,8 +265,8 @@ def _route(logits, k, bias, groups, keep_groups, group_score, score, renormalise
     ids = torch.empty((T, max(int(k), 0)), dtype=torch.int32, device=dev)
     weights = torch.empty((T, max(int(k), 0)), dtype=torch.float32, device=dev)
     load = torch.empty((E,), dtype=torch.int32, device=dev)
-    _On(dev).call(_lib.load().gf_route, C.byref(opts), logits.data_ptr(), t, T, E, ld, b, ids.data_ptr(),
-                  weights.data_ptr(), load.data_ptr())
+    _call(dev, _lib.load().gf_route, C.byref(opts), logits.data_ptr(), t, T, E, ld, b, ids.data_ptr(),
+          weights.data_ptr(), load.data_ptr())
     return ids, weights, load
 
 
@@ -284,7 +278,7 @@ def route(logits, k, bias=None, groups=1, keep_groups=None, group_score="max", s
     Returns Routes; the weights are differentiable with respect to the logits."""
     keep_groups = groups if keep_groups is None else keep_groups
     args = (logits, k, bias, groups, keep_groups, group_score, score, renormalise, scale)
-    if isinstance(logits, _torch().Tensor) and logits.requires_grad and _torch().is_grad_enabled():
+    if isinstance(logits, _need_torch().Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return Routes(*_autograd()[1].apply(*args))
     return Routes(*_route(*args))
 
@@ -293,7 +287,6 @@ def route_grad(logits, ids, dweights, bias=None, score="softmax", renormalise=Tr
     """The gradient of route's weights with respect to the logits, (T, E) in
     the logits' type, from dweights (T, k) float32 and route's ids; bias, score,
     renormalise and scale as in the call of route (gf_route_grad)."""
-    torch = _torch()
     t, T, E, ld = _matrix(logits, "logits")
     if ids.ndim != 2:
         raise ValueError("ids must be (T, k)")
@@ -304,6 +297,6 @@ def route_grad(logits, ids, dweights, bias=None, score="softmax", renormalise=Tr
     b = _vector(bias, (E,), torch.float32, dev, "bias")
     opts = _lib.RouteOpts(k, _choice(_SCORES, score, "score"), 1, 1, 0, int(bool(renormalise)), float(scale))
     out = torch.empty((T, E), dtype=logits.dtype, device=dev)
-    _On(dev).call(_lib.load().gf_route_grad, C.byref(opts), logits.data_ptr(), t, T, E, ld, b, i, g, out.data_ptr(),
-                  E)
+    _call(dev, _lib.load().gf_route_grad, C.byref(opts), logits.data_ptr(), t, T, E, ld, b, i, g, out.data_ptr(),
+          E)
     return out
