@@ -291,35 +291,44 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    auto compute = [&](uint32_t sa, uint32_t sb) {
+    // Values 16 q + 8 h .. of the step in slots sa and sb, into register set q & 1.
+    bf16x8 a[2][MI], b[2][NI];
+    auto read = [&](uint32_t sa, uint32_t sb, auto part) {
+        constexpr uint32_t q = decltype(part)::value, set = q & 1u;
         const uint8_t *la = lds + sa * L::kA, *lb = lds + 3u * L::kA + sb * L::kB;
+        const uint32_t at = r * 128u + ((2u * q + h) ^ (r >> 1 & 7u)) * 16u;
 #pragma unroll
-        for (uint32_t q = 0; q < 4u; ++q) {   // values 16 q + 8 h .. of the step
-            bf16x8 a[MI], b[NI];
-            const uint32_t at = r * 128u + ((2u * q + h) ^ (r >> 1 & 7u)) * 16u;
+        for (int i = 0; i < MI; ++i) a[set][i] = *reinterpret_cast<const bf16x8*>(la + (wm + 32u * i) * 128u + at);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const bf16x8*>(la + (wm + 32u * i) * 128u + at);
-#pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                if constexpr (TR) {
-                    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-                    const uint32_t i = lane & 15u, row = 16u * q + 8u * h + (i >> 2);
-                    const uint32_t u = ((wn + 32u * j) / 16u + (lane >> 4 & 1u)) ^ (i >> 2);
-                    const uint8_t* from = lb + row * (BN * 2u) + u * 32u + (i & 3u) * 8u;
-                    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)from);
-                    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-                        (__attribute__((address_space(3))) bf16x4*)(from + 4u * BN * 2u));
-                    b[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                } else {
-                    b[j] = *reinterpret_cast<const bf16x8*>(lb + (wn + 32u * j) * 128u + at);
-                }
+        for (int j = 0; j < NI; ++j) {
+            if constexpr (TR) {
+                typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+                const uint32_t i = lane & 15u, row = 16u * q + 8u * h + (i >> 2);
+                const uint32_t u = ((wn + 32u * j) / 16u + (lane >> 4 & 1u)) ^ (i >> 2);
+                const uint8_t* from = lb + row * (BN * 2u) + u * 32u + (i & 3u) * 8u;
+                const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)from);
+                const bf16x4 hi =
+                    __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(from + 4u * BN * 2u));
+                b[set][j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            } else {
+                b[set][j] = *reinterpret_cast<const bf16x8*>(lb + (wn + 32u * j) * 128u + at);
             }
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
         }
     };
+    auto multiply = [&](auto part) {
+        constexpr int set = decltype(part)::value & 1;
+        sched_fence();
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[set][j], a[set][i], acc[i][j], 0, 0, 0);
+        sched_fence();
+    };
+    const std::integral_constant<int, 0> q0;
+    const std::integral_constant<int, 1> q1;
+    const std::integral_constant<int, 2> q2;
+    const std::integral_constant<int, 3> q3;
 
     // s1 - s0 >= 1; past the end the last step again, unused
     fetch_a(s0, 0);
@@ -330,16 +339,25 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
     load_b(min(s0 + 1u, s1 - 1u));
     lds_barrier();
     uint32_t sa = 0, sb = 0;
+    read(0, 0, q0);
     for (uint32_t s = s0; s < s1; ++s) {
         wait_vmcnt<0>();                         // the next step: its copies have landed
         write_b(sb ^ 1u);                        // the slots written and copied to are
         const uint32_t to = sa == 0 ? 2u : sa - 1u;
         fetch_a(min(s + 2u, s1 - 1u), to);       // the step before's, read out before the
         load_b(min(s + 2u, s1 - 1u));            // last barrier
-        compute(sa, sb);
+        sched_fence();                           // the loads start here, not where they are used
+        read(sa, sb, q1);
+        multiply(q0);
+        read(sa, sb, q2);
+        multiply(q1);
+        read(sa, sb, q3);
+        multiply(q2);
         lds_barrier();
         sa = sa == 2u ? 0u : sa + 1u;
         sb ^= 1u;
+        read(sa, sb, q0);                        // after the last step: bytes that nothing uses
+        multiply(q3);
     }
     wait_vmcnt<0>();
     lds_barrier();
@@ -385,6 +403,9 @@ uint32_t blocks_for(uint64_t items) { return uint32_t(std::min<uint64_t>((items 
 // or 128, the sum in parts where the tiles leave compute units idle (at least
 // four steps of 64 a part, one part a compute unit, and no more partial sums
 // than 64 MiB).
+// The plan is part of the interface (the workspace's size), so it is made for
+// the chip's compute units, not the current device's.
+constexpr uint64_t kUnits = 256;
 struct RealPlan {
     uint32_t tile, tm, tn, parts, steps, planes;
 };
@@ -392,11 +413,10 @@ RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
     RealPlan r;
     r.planes = dtype == GF_BF16 ? 1u : dtype == GF_F16 ? 2u : 3u;
     r.steps = uint32_t((J + 63u) / 64u);
-    const uint64_t big = ((M + 255u) / 256u) * ((N + 255u) / 256u);
-    r.tile = big >= 192u ? 256u : 128u;
+    r.tile = large_tiles(M, N, kUnits) ? 256u : 128u;
     r.tm = uint32_t((M + r.tile - 1u) / r.tile), r.tn = uint32_t((N + r.tile - 1u) / r.tile);
     const uint64_t tiles = uint64_t(r.tm) * r.tn;
-    uint64_t parts = std::min<uint64_t>(256u / tiles, uint64_t(r.steps) * r.planes / 4u);
+    uint64_t parts = std::min<uint64_t>(kUnits / tiles, uint64_t(r.steps) * r.planes / 4u);
     parts = std::min<uint64_t>(parts, (64u << 20) / (M * N * 4u));
     r.parts = uint32_t(std::max<uint64_t>(parts, 1u));
     return r;

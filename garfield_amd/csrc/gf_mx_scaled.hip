@@ -328,12 +328,11 @@ hipError_t launch_mx_product_mx(const gf_mx_rows& x, const gf_mx_rows& w, const 
     const uint64_t M = x.rows, N = w.rows;
     const uint32_t S = mx_chunks(w.K);
     if (M <= 16) return S >= 8 ? direct<1, 1, 1, 8>(x, w, out, st) : direct<1, 1, 1, 1>(x, w, out, st);
-    if (S >= 4) {
-        const uint64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
-        if (big >= 192 && S < 1u << 18) return tile<256, 256, 2, 4>(x, w, out, st);
-        if (mid >= 128 && S < 1u << 18) return tile<128, 128, 2, 2>(x, w, out, st);
-        return direct<4, 4, 1, 4>(x, w, out, st);
+    if (S >= 4 && S < 1u << 18) {
+        if (large_tiles(M, N, compute_units())) return tile<256, 256, 2, 4>(x, w, out, st);
+        if (((M + 127) / 128) * ((N + 127) / 128) >= 128) return tile<128, 128, 2, 2>(x, w, out, st);
     }
+    if (S >= 4) return direct<4, 4, 1, 4>(x, w, out, st);
     return direct<4, 4, 4, 1>(x, w, out, st);
 }
 
