@@ -194,10 +194,15 @@ __global__ __launch_bounds__(64 * WK) void k_mx_few(const ElemT<DT>* x, uint32_t
 
 // ---- tiles through LDS -----------------------------------------------------
 // A block has a tile of BM real rows x BN columns of the result, 64 values of
-// the sum a step, its VM x VN waves equal parts of the tile.  The real side
-// comes as planes, by copies straight to LDS, two steps ahead (three slots);
-// the 4-bit side through registers, one block of 32 values a thread, decoded
-// on its way to LDS, one step ahead (two slots).
+// the sum a step, its VM x VN waves equal parts of the tile.  The 4-bit side
+// comes through registers, one block of 32 values a thread, decoded on its way
+// to LDS, loaded one step ahead (two slots).  A real side in bfloat16 (or in
+// planes, one after the other) comes by copies straight to LDS, two steps ahead
+// (three slots); one in binary16 or fp32 through registers, split into its
+// planes on its way, one step ahead (two slots): a small result is then one
+// launch, and the planes share what is read and decoded of the other side.  A
+// step has four parts; a part's operands are read from LDS while the part before
+// it is multiplied, across steps too.
 // Columns are rows of w (TR = false: the product) or positions in w's rows
 // (TR = true: the gradient, whose sum runs over w's rows).  Slots of the real
 // side, and of w without TR, have rows of 64 values, 128 bytes; their 16-byte
@@ -210,27 +215,31 @@ __global__ __launch_bounds__(64 * WK) void k_mx_few(const ElemT<DT>* x, uint32_t
 // The sum may be cut into `parts`, each block then writing its own in fp32 to
 // a workspace (out, rows of ldo, a part every M ldo), which k_mx_join adds up
 // in order.
-template <int BM, int BN, int OT, bool TR>
+template <int DT, int BM, int BN, int OT, bool TR>
 struct RealLds {
-    static constexpr uint32_t kA = BM * 128u, kB = BN * 128u, kBytes = 3u * kA + 2u * kB;
+    static constexpr bool kSplit = DT != GF_BF16;
+    static constexpr uint32_t kPlane = BM * 128u, kA = kPlane * kPlanes<DT>, kB = BN * 128u, kSlots = kSplit ? 2u : 3u;
+    static constexpr uint32_t kBytes = kSlots * kA + 2u * kB;
     static constexpr uint32_t kCols = 32u;
     using P = Piece<OT, kCols>;
 };
 
 struct RealArgs {
-    const uint16_t* a;      // planes of the real side
-    uint64_t lda, step;     // distance of its rows and steps, in elements
-    uint32_t planes, M, J;  // J: length of the sum in steps of 64
+    const void* a;       // the real side
+    uint64_t lda, step;  // distance of its rows and, in bfloat16, steps, in elements
+    uint32_t M, J;       // its rows, and their length
+    uint32_t planes;     // in bfloat16: planes one after the other
     gf_mx_rows w;
-    uint32_t S, N;          // N: columns of the result
+    uint32_t S, N;       // N: columns of the result
     uint32_t tm, tn, parts;
 };
 
-template <int BM, int BN, int VM, int VN, int OT, bool TR>
+template <int DT, int BM, int BN, int VM, int VN, int OT, bool TR>
 __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>* out, uint64_t ldo) {
-    using L = RealLds<BM, BN, OT, TR>;
+    using L = RealLds<DT, BM, BN, OT, TR>;
     using Pc = typename L::P;
-    constexpr uint32_t TH = 64u * VM * VN, kPer = BM * 8u / TH;
+    constexpr int P = kPlanes<DT>;
+    constexpr uint32_t TH = 64u * VM * VN, kPer = BM * 8u / TH;   // 8-value pieces of the real side a thread and step
     constexpr int MI = BM / VM / 32, NI = BN / VN / 32;
     static_assert(BN * 2u == TH && VM * VN * Pc::kBytes <= L::kBytes, "");
     __shared__ __align__(16) uint8_t lds[L::kBytes];
@@ -242,21 +251,64 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
     uint32_t m0, n0;
     tile_of(id % tiles, p.tm, p.tn, 4u, m0, n0);
     m0 *= BM, n0 *= BN;
-    const uint32_t total = p.J * p.planes;   // every plane goes over all of w
+    const uint32_t steps = (p.J + 63u) / 64u, total = steps * p.planes;
     const uint32_t s0 = uint32_t(uint64_t(total) * cut / p.parts), s1 = uint32_t(uint64_t(total) * (cut + 1u) / p.parts);
 
-    // rows beyond the end repeat the last one; their sums are not stored
-    uint32_t oa[kPer];
-    const uint8_t* pa = reinterpret_cast<const uint8_t*>(p.a + uint64_t(m0) * p.lda);
+    // The thread's pieces: row i (TH / 8) + tid / 8, place tid & 7.  Rows beyond
+    // the end repeat the last one; their sums are not stored.
+    const uint32_t piece_of = (tid & 7u) ^ (tid >> 4 & 7u);
+    uint32_t oa[kPer];                                   // bfloat16: byte offsets for the copies
+    const ElemT<DT>* ra[kPer];                           // else the rows,
+    constexpr uint32_t kRaw = sizeof(ElemT<DT>) / 2u;    // and eight values of each as loaded
+    uint4 raw[kPer][kRaw];
+    const uint8_t* pa = static_cast<const uint8_t*>(p.a) + uint64_t(m0) * p.lda * 2u;
 #pragma unroll
     for (uint32_t i = 0; i < kPer; ++i) {
-        const uint32_t row = i * (TH / 8u) + tid / 8u;
-        oa[i] = uint32_t(min(row, p.M - 1u - m0) * uint32_t(p.lda * 2u)) + ((tid & 7u) ^ (tid >> 4 & 7u)) * 16u;
+        const uint32_t row = min(i * (TH / 8u) + tid / 8u, p.M - 1u - m0);
+        if constexpr (L::kSplit)
+            ra[i] = static_cast<const ElemT<DT>*>(p.a) + uint64_t(m0 + row) * p.lda;
+        else
+            oa[i] = row * uint32_t(p.lda * 2u) + piece_of * 16u;
     }
-    auto fetch_a = [&](uint32_t s, uint32_t slot) {
-        const uint8_t* at = pa + uint64_t(s) * p.step * 2u;
+    auto load_a = [&](uint32_t s, uint32_t slot) {
+        if constexpr (!L::kSplit) {
+            const uint8_t* at = pa + uint64_t(s) * p.step * 2u;
 #pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) lds_copy16(at, oa[i], base + slot * L::kA + i * TH * 16u + wave * 1024u);
+            for (uint32_t i = 0; i < kPer; ++i) lds_copy16(at, oa[i], base + slot * L::kA + i * TH * 16u + wave * 1024u);
+        } else {
+            const uint32_t k = s * 64u + piece_of * 8u;
+            if (k + 8u <= p.J) {
+#pragma unroll
+                for (uint32_t i = 0; i < kPer; ++i)
+#pragma unroll
+                    for (uint32_t q = 0; q < kRaw; ++q) raw[i][q] = load16(reinterpret_cast<const uint8_t*>(ra[i] + k) + q * 16u);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < kPer; ++i) {
+                    ElemT<DT> e[8];
+#pragma unroll
+                    for (uint32_t c = 0; c < 8u; ++c) e[c] = k + c < p.J ? ra[i][k + c] : ElemT<DT>(0.0f);
+                    __builtin_memcpy(raw[i], e, sizeof(e));
+                }
+            }
+        }
+    };
+    auto write_a = [&](uint32_t slot) {
+        if constexpr (L::kSplit) {
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i) {
+                ElemT<DT> e[8];
+                __builtin_memcpy(e, raw[i], sizeof(e));
+                float v[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] = float(e[c]);
+                uint4 plane[P];
+                split8<P>(v, plane);
+#pragma unroll
+                for (int q = 0; q < P; ++q)
+                    *reinterpret_cast<uint4*>(lds + slot * L::kA + q * L::kPlane + (i * TH + tid) * 16u) = plane[q];
+            }
+        }
     };
     // A thread's block: row n0 + tid / 2, half tid & 1 of the step; with TR row
     // tid / (BN / 32) of the step, block tid % (BN / 32) of the tile's columns.
@@ -264,14 +316,14 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
     uint4 code;
     uint32_t byte;
     auto load_b = [&](uint32_t s) {
-        const uint32_t j = s % p.J;
+        const uint32_t j = s % steps;
         const uint64_t row = TR ? min(j * 64u + tid / kAcross, uint32_t(p.w.rows) - 1u) : min(n0 + tid / 2u, p.N - 1u);
         const uint64_t blk = row * (4u * p.S) + (TR ? min(n0 / 32u + tid % kAcross, 4u * p.S - 1u) : j * 2u + (tid & 1u));
         code = reinterpret_cast<const uint4*>(p.w.codes)[blk];
         byte = p.w.scales[blk];
     };
     auto write_b = [&](uint32_t slot) {
-        uint8_t* to = lds + 3u * L::kA + slot * L::kB;
+        uint8_t* to = lds + L::kSlots * L::kA + slot * L::kB;
         const float scale = mx_scale(byte);
         const uint32_t word[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
@@ -292,13 +344,16 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     // Values 16 q + 8 h .. of the step in slots sa and sb, into register set q & 1.
-    bf16x8 a[2][MI], b[2][NI];
+    bf16x8 a[2][P][MI], b[2][NI];
     auto read = [&](uint32_t sa, uint32_t sb, auto part) {
         constexpr uint32_t q = decltype(part)::value, set = q & 1u;
-        const uint8_t *la = lds + sa * L::kA, *lb = lds + 3u * L::kA + sb * L::kB;
+        const uint8_t *la = lds + sa * L::kA, *lb = lds + L::kSlots * L::kA + sb * L::kB;
         const uint32_t at = r * 128u + ((2u * q + h) ^ (r >> 1 & 7u)) * 16u;
 #pragma unroll
-        for (int i = 0; i < MI; ++i) a[set][i] = *reinterpret_cast<const bf16x8*>(la + (wm + 32u * i) * 128u + at);
+        for (int c = 0; c < P; ++c)
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+                a[set][c][i] = *reinterpret_cast<const bf16x8*>(la + c * L::kPlane + (wm + 32u * i) * 128u + at);
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
             if constexpr (TR) {
@@ -319,10 +374,12 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
         constexpr int set = decltype(part)::value & 1;
         sched_fence();
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+        for (int c = 0; c < P; ++c)
 #pragma unroll
-            for (int j = 0; j < NI; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[set][j], a[set][i], acc[i][j], 0, 0, 0);
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[set][j], a[set][c][i], acc[i][j], 0, 0, 0);
         sched_fence();
     };
     const std::integral_constant<int, 0> q0;
@@ -330,23 +387,11 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
     const std::integral_constant<int, 2> q2;
     const std::integral_constant<int, 3> q3;
 
-    // s1 - s0 >= 1; past the end the last step again, unused
-    fetch_a(s0, 0);
-    load_b(s0);
-    wait_vmcnt<0>();
-    write_b(0);
-    fetch_a(min(s0 + 1u, s1 - 1u), 1);
-    load_b(min(s0 + 1u, s1 - 1u));
-    lds_barrier();
+    // The step in slots sa and sb, whose first part has been read; the next step
+    // lies in the slots behind (after the last one: bytes that nothing uses).
     uint32_t sa = 0, sb = 0;
-    read(0, 0, q0);
-    for (uint32_t s = s0; s < s1; ++s) {
-        wait_vmcnt<0>();                         // the next step: its copies have landed
-        write_b(sb ^ 1u);                        // the slots written and copied to are
-        const uint32_t to = sa == 0 ? 2u : sa - 1u;
-        fetch_a(min(s + 2u, s1 - 1u), to);       // the step before's, read out before the
-        load_b(min(s + 2u, s1 - 1u));            // last barrier
-        sched_fence();                           // the loads start here, not where they are used
+    auto step = [&]() {
+        sched_fence();   // loads above start there, not where they are used
         read(sa, sb, q1);
         multiply(q0);
         read(sa, sb, q2);
@@ -354,11 +399,57 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
         read(sa, sb, q3);
         multiply(q2);
         lds_barrier();
-        sa = sa == 2u ? 0u : sa + 1u;
+        sa = sa + 1u == L::kSlots ? 0u : sa + 1u;
         sb ^= 1u;
-        read(sa, sb, q0);                        // after the last step: bytes that nothing uses
+        read(sa, sb, q0);
         multiply(q3);
+    };
+    auto load = [&](uint32_t s) {
+        load_a(s, sa == 0 ? 2u : sa - 1u);   // (bfloat16) two slots on
+        load_b(s);
+    };
+    auto landed = [&]() {   // the next step's; its slots are those of the step before,
+        wait_vmcnt<0>();    // read out before the last barrier
+        write_a(sa ^ 1u);
+        write_b(sb ^ 1u);
+    };
+
+    // n >= 1 steps.  The first two are loaded together: a short sum waits for
+    // memory once.
+    const uint32_t n = s1 - s0;
+    {
+        const uint32_t next = min(s0 + 1u, s1 - 1u);
+        load_a(s0, 0);
+        load_b(s0);
+        if constexpr (!L::kSplit) load_a(next, 1);
+        uint4 raw0[kPer][kRaw];
+        __builtin_memcpy(raw0, raw, sizeof(raw));
+        const uint4 code0 = code;
+        const uint32_t byte0 = byte;
+        if constexpr (L::kSplit) load_a(next, 1);
+        load_b(next);
+        wait_vmcnt<0>();
+        write_a(1);
+        write_b(1);
+        __builtin_memcpy(raw, raw0, sizeof(raw));
+        code = code0, byte = byte0;
+        write_a(0);
+        write_b(0);
     }
+    lds_barrier();
+    if (n > 2u) load(s0 + 2u);
+    read(0, 0, q0);
+    step();
+    for (uint32_t s = s0 + 1u; s + 2u < s1; ++s) {
+        landed();
+        load(s + 2u);
+        step();
+    }
+    if (n > 2u) {
+        landed();
+        step();
+    }
+    if (n > 1u) step();
     wait_vmcnt<0>();
     lds_barrier();
     ElemT<OT>* o = out + uint64_t(cut) * p.M * ldo;
@@ -399,30 +490,35 @@ __global__ __launch_bounds__(256) void k_mx_zero(uint64_t M, uint32_t N, ElemT<O
 
 uint32_t blocks_for(uint64_t items) { return uint32_t(std::min<uint64_t>((items + 255u) / 256u, 1u << 20)); }
 
-// How a product of M real rows of J values with N columns runs: tiles of 256
-// or 128, the sum in parts where the tiles leave compute units idle (at least
-// four steps of 64 a part, one part a compute unit, and no more partial sums
-// than 64 MiB).
-// The plan is part of the interface (the workspace's size), so it is made for
-// the chip's compute units, not the current device's.
+// How a product of M real rows of J values with N columns runs: the tile, and
+// the sum in parts where the tiles leave compute units idle (at least four
+// steps of 64 a part, one part a compute unit, and no more partial sums than 64
+// MiB).  The plan is part of the interface (the workspace's size), so it is made
+// for the chip's compute units, not the current device's.
 constexpr uint64_t kUnits = 256;
 struct RealPlan {
-    uint32_t tile, tm, tn, parts, steps, planes;
+    bool large, planes;   // tiles of 256; the real side as planes in the workspace
+    uint32_t tm, tn, parts;
 };
 RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
     RealPlan r;
-    r.planes = dtype == GF_BF16 ? 1u : dtype == GF_F16 ? 2u : 3u;
-    r.steps = uint32_t((J + 63u) / 64u);
-    r.tile = large_tiles(M, N, kUnits) ? 256u : 128u;
-    r.tm = uint32_t((M + r.tile - 1u) / r.tile), r.tn = uint32_t((N + r.tile - 1u) / r.tile);
-    const uint64_t tiles = uint64_t(r.tm) * r.tn;
-    uint64_t parts = std::min<uint64_t>(kUnits / tiles, uint64_t(r.steps) * r.planes / 4u);
+    r.large = large_tiles(M, N, kUnits);
+    // Binary16 and fp32 pay for planes only where tiles are large.  fp32, planes
+    // against splitting in the kernel: 4096 x 8192 x 4096 735 us against 1008,
+    // 2048 x 4096 x 4096 268 against 292, 2048 x 2048 x 4096 169 against 151, the
+    // gradient of 500 queries over 60000 rows of 128 107 against 47.
+    r.planes = dtype == GF_BF16 || r.large;
+    const uint64_t tm = r.large ? 256u : r.planes ? 128u : 64u, tn = r.large ? 256u : 128u;
+    r.tm = uint32_t((M + tm - 1u) / tm), r.tn = uint32_t((N + tn - 1u) / tn);
+    // two of the smaller tiles share a compute unit
+    uint64_t parts = std::min<uint64_t>((r.planes ? 1u : 2u) * kUnits / (uint64_t(r.tm) * r.tn), (J + 63u) / 64u / 4u);
     parts = std::min<uint64_t>(parts, (64u << 20) / (M * N * 4u));
     r.parts = uint32_t(std::max<uint64_t>(parts, 1u));
     return r;
 }
-// Whether the real side can be read in place: bfloat16 rows of whole steps,
-// aligned for the copies.
+uint32_t planes_of(int32_t dtype) { return dtype == GF_BF16 ? 1u : dtype == GF_F16 ? 2u : 3u; }
+// Whether a bfloat16 side can be read in place: rows of whole steps, aligned
+// for the copies.
 bool in_place(const MatIn& a, uint64_t J) {
     return a.dtype == GF_BF16 && J % 64u == 0 && a.ld % 8u == 0 && reinterpret_cast<uintptr_t>(a.p) % 16u == 0 && a.ld < 1u << 22;
 }
@@ -431,29 +527,33 @@ template <bool TR>
 hipError_t real_product(const MatIn& a, uint64_t J, const gf_mx_rows& w, uint64_t N, const MatOut& out, void* ws,
                         hipStream_t st) {
     const RealPlan pl = real_plan(a.dtype, a.rows, N, J);
-    RealArgs p = {static_cast<const uint16_t*>(a.p), a.ld, 64, pl.planes, uint32_t(a.rows), pl.steps, w, mx_chunks(w.K), uint32_t(N),
-                  pl.tm, pl.tn, pl.parts};
+    RealArgs p = {a.p, a.ld, 64, uint32_t(a.rows), uint32_t(J), 1u, w, mx_chunks(w.K), uint32_t(N), pl.tm, pl.tn, pl.parts};
     uint8_t* at = static_cast<uint8_t*>(ws);
-    if (!in_place(a, J)) {
-        p.a = reinterpret_cast<const uint16_t*>(at), p.lda = 64, p.step = a.rows * 64u;
+    if (pl.planes && !in_place(a, J)) {
+        const uint32_t steps = uint32_t((J + 63u) / 64u);
+        p.a = at, p.lda = 64, p.step = a.rows * 64u, p.planes = planes_of(a.dtype);
         const hipError_t e = by_type(a.dtype, [&](auto dt) {
             constexpr int DT = decltype(dt)::value;
-            hipLaunchKernelGGL(k_mx_planes<DT>, dim3(blocks_for(a.rows * pl.steps * 8u)), 256, 0, st,
-                               static_cast<const ElemT<DT>*>(a.p), a.rows, uint32_t(J), a.ld, pl.steps,
+            hipLaunchKernelGGL(k_mx_planes<DT>, dim3(blocks_for(a.rows * steps * 8u)), 256, 0, st,
+                               static_cast<const ElemT<DT>*>(a.p), a.rows, uint32_t(J), a.ld, steps,
                                reinterpret_cast<uint16_t*>(at));
             return hipGetLastError();
         });
         if (e != hipSuccess) return e;
-        at += a.rows * pl.steps * pl.planes * 128u;
+        at += a.rows * steps * p.planes * 128u;
     }
     auto run = [&](auto ot, void* to, uint64_t ldo) {
         constexpr int OT = decltype(ot)::value;
-        if (pl.tile == 256u)
-            hipLaunchKernelGGL((k_mx_real<256, 256, 2, 4, OT, TR>), dim3(pl.tm * pl.tn * pl.parts), 512, 0, st, p,
-                               static_cast<ElemT<OT>*>(to), ldo);
+        ElemT<OT>* o = static_cast<ElemT<OT>*>(to);
+        const dim3 grid(pl.tm * pl.tn * pl.parts);
+        if (pl.large)
+            hipLaunchKernelGGL((k_mx_real<GF_BF16, 256, 256, 2, 4, OT, TR>), grid, 512, 0, st, p, o, ldo);
+        else if (a.dtype == GF_BF16)
+            hipLaunchKernelGGL((k_mx_real<GF_BF16, 128, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
+        else if (a.dtype == GF_F16)
+            hipLaunchKernelGGL((k_mx_real<GF_F16, 64, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
         else
-            hipLaunchKernelGGL((k_mx_real<128, 128, 2, 2, OT, TR>), dim3(pl.tm * pl.tn * pl.parts), 256, 0, st, p,
-                               static_cast<ElemT<OT>*>(to), ldo);
+            hipLaunchKernelGGL((k_mx_real<GF_F32, 64, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
         return hipGetLastError();
     };
     if (pl.parts == 1u) return by_type(out.dtype, [&](auto ot) { return run(ot, out.p, out.ld); });
@@ -510,8 +610,9 @@ size_t mx_workspace(int32_t kind, int32_t dtype, uint64_t M, uint64_t rows, uint
     if (kind == 1 || !M || !rows || (kind == 0 && M <= kFew)) return 0;
     const uint64_t J = kind == 2 ? rows : K, N = kind == 2 ? K : rows;
     const RealPlan pl = real_plan(dtype, M, N, J);
-    // room for the planes whether or not the real side can be read in place
-    return size_t(pl.steps) * 128u * pl.planes * M + (pl.parts > 1u ? size_t(pl.parts) * M * N * 4u : 0u);
+    // bfloat16: room for the rows by steps, whether or not they can be read in place
+    return (pl.planes ? size_t((J + 63u) / 64u) * 128u * planes_of(dtype) * M : 0u) +
+           (pl.parts > 1u ? size_t(pl.parts) * M * N * 4u : 0u);
 }
 
 }  // namespace gf
