@@ -45,6 +45,12 @@ struct __attribute__((packed, aligned(1))) Bytes16 {
     uint4 v;
 };
 __device__ __forceinline__ uint4 load16(const void* p) { return static_cast<const Bytes16*>(p)->v; }
+// The same for what is read once.
+__device__ __forceinline__ uint4 load16_once(const void* p) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(1)));
+    const u32x4 v = __builtin_nontemporal_load(static_cast<const u32x4*>(p));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
 __device__ __forceinline__ void store16(void* p, uint4 v) { static_cast<Bytes16*>(p)->v = v; }
 
 // Workgroups go to the eight XCDs in turn, each with an L2 of its own: ids are
