@@ -512,7 +512,7 @@ RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
     r.tm = uint32_t((M + tm - 1u) / tm), r.tn = uint32_t((N + tn - 1u) / tn);
     // two of the smaller tiles share a compute unit
     uint64_t parts = std::min<uint64_t>((r.planes ? 1u : 2u) * kUnits / (uint64_t(r.tm) * r.tn), (J + 63u) / 64u / 4u);
-    parts = std::min<uint64_t>(parts, (64u << 20) / (M * N * 4u));
+    parts = std::min<uint64_t>(parts, (16u << 20) / (M * N));
     r.parts = uint32_t(std::max<uint64_t>(parts, 1u));
     return r;
 }
@@ -527,6 +527,7 @@ template <bool TR>
 hipError_t real_product(const MatIn& a, uint64_t J, const gf_mx_rows& w, uint64_t N, const MatOut& out, void* ws,
                         hipStream_t st) {
     const RealPlan pl = real_plan(a.dtype, a.rows, N, J);
+    if (!grid_fits(uint64_t(pl.tm) * pl.tn * pl.parts, 512u)) return hipErrorInvalidConfiguration;
     RealArgs p = {a.p, a.ld, 64, uint32_t(a.rows), uint32_t(J), 1u, w, mx_chunks(w.K), uint32_t(N), pl.tm, pl.tn, pl.parts};
     uint8_t* at = static_cast<uint8_t*>(ws);
     if (pl.planes && !in_place(a, J)) {
@@ -578,6 +579,7 @@ hipError_t launch_mx_product(const MatIn& x, const gf_mx_rows& w, const MatOut& 
             constexpr int DT = decltype(dt)::value, OT = decltype(ot)::value;
             auto go = [&](auto nt, auto wk) {
                 constexpr int NT = decltype(nt)::value, WK = decltype(wk)::value;
+                if (!grid_fits((w.rows + 16u * NT - 1u) / (16u * NT), 64u * WK)) return hipErrorInvalidConfiguration;
                 hipLaunchKernelGGL((k_mx_few<DT, NT, WK, OT>), dim3(uint32_t((w.rows + 16u * NT - 1u) / (16u * NT))), 64 * WK, 0,
                                    st, static_cast<const ElemT<DT>*>(x.p), uint32_t(x.rows), x.ld, w, S,
                                    static_cast<ElemT<OT>*>(out.p), out.ld);

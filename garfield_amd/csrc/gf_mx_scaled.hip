@@ -302,6 +302,7 @@ template <int MT, int NT, int WN, int WK>
 hipError_t direct(const gf_mx_rows& x, const gf_mx_rows& w, const MatOut& out, hipStream_t st) {
     const uint32_t S = mx_chunks(w.K);
     const uint32_t tm = uint32_t((x.rows + 16u * MT - 1u) / (16u * MT)), tn = uint32_t((w.rows + 16u * NT * WN - 1u) / (16u * NT * WN));
+    if (!grid_fits(uint64_t(tm) * tn, 64u * WN * WK)) return hipErrorInvalidConfiguration;
     return by_type(out.dtype, [&](auto ot) {
         constexpr int OT = decltype(ot)::value;
         hipLaunchKernelGGL((k_mx_direct<MT, NT, WN, WK, OT>), dim3(tm * tn), 64 * WN * WK, 0, st, x, w, S, tm, tn,
@@ -312,6 +313,7 @@ hipError_t direct(const gf_mx_rows& x, const gf_mx_rows& w, const MatOut& out, h
 template <int BM, int BN, int VM, int VN>
 hipError_t tile(const gf_mx_rows& x, const gf_mx_rows& w, const MatOut& out, hipStream_t st) {
     const uint32_t tm = uint32_t((x.rows + BM - 1u) / BM), tn = uint32_t((w.rows + BN - 1u) / BN);
+    if (!grid_fits(uint64_t(tm) * tn, 64u * VM * VN)) return hipErrorInvalidConfiguration;
     return by_type(out.dtype, [&](auto ot) {
         constexpr int OT = decltype(ot)::value;
         // as many blocks as the chip's LDS holds at once

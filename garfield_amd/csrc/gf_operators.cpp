@@ -71,6 +71,11 @@ void check_route(const gf_route_opts* o, uint64_t E, bool choose) {
     GF_REQUIRE(o->k <= o->keep_groups * (E / o->groups), GF_E_ARG, "k exceeds the entries of keep_groups groups");
 }
 
+void launched(hipError_t e) {
+    GF_REQUIRE(e != hipErrorInvalidConfiguration, GF_E_UNSUPPORTED, "sizes need more workgroups than a launch has");
+    GF_HIP(e);
+}
+
 template <class T>
 void check_pointer(const T* p, bool needed, const char* what) {
     GF_REQUIRE(p || !needed, GF_E_ARG, std::string(what) + ": null pointer");
@@ -86,7 +91,7 @@ gf_status gf_mx_quantise(const void* x, int32_t dtype, uint64_t rows, uint32_t K
         const gf_mx_rows out = {codes, scales, rows, K};
         check_rows(&out, "out");
         if (!rows) return;
-        GF_HIP(gf::launch_mx_quantise({x, dtype, rows, ld}, K, codes, scales, hipStream_t(stream)));
+        launched(gf::launch_mx_quantise({x, dtype, rows, ld}, K, codes, scales, hipStream_t(stream)));
     });
 }
 
@@ -95,7 +100,7 @@ gf_status gf_mx_dequantise(const gf_mx_rows* w, int32_t dtype, void* out, uint64
         check_rows(w, "w");
         check_matrix(out, dtype, w->rows, w->K, ldo, "out");
         if (!w->rows) return;
-        GF_HIP(gf::launch_mx_dequantise(*w, {out, dtype, ldo}, hipStream_t(stream)));
+        launched(gf::launch_mx_dequantise(*w, {out, dtype, ldo}, hipStream_t(stream)));
     });
 }
 
@@ -107,7 +112,7 @@ gf_status gf_mx_product(const void* x, int32_t dtype, uint64_t M, uint64_t ldx, 
         check_matrix(out, out_dtype, M, w->rows, ldo, "out");
         check_workspace(0, dtype, M, *w, workspace, workspace_bytes);
         if (!M || !w->rows) return;
-        GF_HIP(gf::launch_mx_product({x, dtype, M, ldx}, *w, {out, out_dtype, ldo}, workspace, hipStream_t(stream)));
+        launched(gf::launch_mx_product({x, dtype, M, ldx}, *w, {out, out_dtype, ldo}, workspace, hipStream_t(stream)));
     });
 }
 
@@ -120,7 +125,7 @@ gf_status gf_mx_product_mx(const gf_mx_rows* x, const gf_mx_rows* w, int32_t out
         check_matrix(out, out_dtype, x->rows, w->rows, ldo, "out");
         check_workspace(1, GF_F32, x->rows, *w, workspace, workspace_bytes);
         if (!x->rows || !w->rows) return;
-        GF_HIP(gf::launch_mx_product_mx(*x, *w, {out, out_dtype, ldo}, workspace, hipStream_t(stream)));
+        launched(gf::launch_mx_product_mx(*x, *w, {out, out_dtype, ldo}, workspace, hipStream_t(stream)));
     });
 }
 
@@ -133,7 +138,7 @@ gf_status gf_mx_product_grad(const void* dy, int32_t dtype, uint64_t M, uint64_t
         check_matrix(dx, out_dtype, M, w->K, ldo, "dx");
         check_workspace(2, dtype, M, *w, workspace, workspace_bytes);
         if (!M) return;
-        GF_HIP(gf::launch_mx_product_grad({dy, dtype, M, ldy}, *w, {dx, out_dtype, ldo}, workspace,
+        launched(gf::launch_mx_product_grad({dy, dtype, M, ldy}, *w, {dx, out_dtype, ldo}, workspace,
                                           hipStream_t(stream)));
     });
 }
@@ -157,7 +162,7 @@ gf_status gf_route(const gf_route_opts* opts, const void* logits, int32_t dtype,
         check_pointer(ids, T != 0, "ids");
         check_pointer(weights, T != 0, "weights");
         check_pointer(load, false, "load");
-        GF_HIP(gf::launch_route(*opts, {logits, dtype, T, ld}, E, bias, ids, weights, load, hipStream_t(stream)));
+        launched(gf::launch_route(*opts, {logits, dtype, T, ld}, E, bias, ids, weights, load, hipStream_t(stream)));
     });
 }
 
@@ -172,7 +177,7 @@ gf_status gf_route_grad(const gf_route_opts* opts, const void* logits, int32_t d
         check_pointer(ids, T != 0, "ids");
         check_pointer(dweights, T != 0, "dweights");
         if (!T) return;
-        GF_HIP(gf::launch_route_grad(*opts, {logits, dtype, T, ld}, E, bias, ids, dweights, {dlogits, dtype, ldd},
+        launched(gf::launch_route_grad(*opts, {logits, dtype, T, ld}, E, bias, ids, dweights, {dlogits, dtype, ldd},
                                      hipStream_t(stream)));
     });
 }

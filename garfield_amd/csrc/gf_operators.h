@@ -21,6 +21,10 @@ struct MatOut {
     uint64_t ld;
 };
 
+// Launchers return hipErrorInvalidConfiguration for sizes that need more
+// threads than a launch has.
+inline bool grid_fits(uint64_t blocks, uint32_t threads) { return blocks <= 0xFFFFFFFFu / threads; }
+
 inline uint32_t mx_chunks(uint32_t K) { return (K >> 7) + ((K & 127u) != 0); }  // of 128 values a row
 
 hipError_t launch_mx_quantise(const MatIn& x, uint32_t K, uint8_t* codes, uint8_t* scales, hipStream_t st);

@@ -320,9 +320,10 @@ __global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_
         auto rank_of = [&](float first_best, float second_best) {
             return first_best + (o.group_score == GF_GROUP_TOP2 && second_best > kNone ? second_best : 0.0f);
         };
-        // a rank is the sum of two keys at most, each |key| below |rank| + top
+        // a rank is the sum of two keys at most; no key is below -top, so neither
+        // is beyond |rank| + top
         auto too_close = [&](float low, float high) {
-            return by_score && high > kNone && low - high <= 2.0f * (off(low) + off(high) + rel * top);
+            return by_score && high > kNone && low - high <= 2.0f * (off(low) + off(high) + 2.0f * rel * top);
         };
         if (o.groups == 1u || whole) {
 #pragma unroll

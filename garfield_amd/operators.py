@@ -201,6 +201,7 @@ def _autograd():
                 return _product(x, w, dtype)
 
             @staticmethod
+            @torch.autograd.function.once_differentiable
             def backward(ctx, dy):
                 if dy.ndim == 2 and dy.shape[1] > 1 and dy.stride(1) != 1 or dy.stride(0) < dy.shape[1]:
                     dy = dy.contiguous()
@@ -217,6 +218,7 @@ def _autograd():
                 return ids, weights, load
 
             @staticmethod
+            @torch.autograd.function.once_differentiable
             def backward(ctx, _ids, dweights, _load):
                 logits, ids, bias = ctx.saved_tensors
                 d = route_grad(logits, ids, dweights.contiguous(), bias=bias, **ctx.how)

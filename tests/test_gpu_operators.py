@@ -467,3 +467,13 @@ def test_autograd():
     x.grad = None
     gf.mx_product(x, w).t().matmul(torch.ones(7, 3, device="cuda")).sum().backward()   # a transposed dy
     _close(x.grad, 3 * np.ones((7, 60)) @ wv, orc.product_bound(3 * np.ones((7, 60)), np.ascontiguousarray(wv.T), "float32"), "dy^T")
+
+
+def test_gradients_of_gradients_are_refused():
+    _case("second derivatives")
+    w, _ = _mx(20, 64, 1)
+    x = _rows(3, 64, torch.float32, 2, spread=False).requires_grad_()
+    for y in (gf.mx_product(x, w).square().sum(), gf.route(x, 4).weights.square().sum()):
+        (d,) = torch.autograd.grad(y, x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            d.sum().backward()

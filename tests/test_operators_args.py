@@ -67,6 +67,15 @@ def test_product_mx_refuses():
     assert _status("gf_mx_product_mx", _mx(scales=None), _mx(), 0, P, 8, None, 0) == ARG
 
 
+def test_more_workgroups_than_a_launch_has():
+    """Refused on the host: 2^40 tiles."""
+    far = 1 << 28
+    assert _status("gf_mx_product_mx", _mx(far, 32), _mx(far, 32), 0, P, far, None, 0) == UNSUPPORTED
+    n = C.c_size_t()
+    assert _lib.load().gf_mx_product_workspace(0, 2, far, far, 64, C.byref(n)) == 0
+    assert _status("gf_mx_product", P, 2, far, 64, _mx(far, 64), 0, P, far, P, n.value) == UNSUPPORTED
+
+
 def test_workspace_is_checked():
     """A call whose workspace is too small, missing or misaligned is refused."""
     n = C.c_size_t()
