@@ -1,10 +1,10 @@
 // Routing of queries (tokens) to cells (experts) and its gradient (gfx950,
 // wave64).  The definition is at gf_route in the header.
 //
-// Both are small passes over T x E logits.  Sixteen lanes hold a row, so a wave
-// works on four; all they exchange goes through data-parallel moves within
-// their sixteen lanes or a few words of LDS of their own wave, and no barrier
-// stands between the load of a row and its result.
+// Both are small passes over T x E logits.  Sixteen lanes hold a row of up to 256
+// entries, so a wave works on four; a longer row takes the whole wave.  All that
+// lanes exchange goes through data-parallel moves or a few words of LDS of their
+// own wave, and no barrier stands between the load of a row and its result.
 //
 // Which entries are chosen must not hang on the last bit of a 32-bit
 // exponential.  Keys (score + bias) are computed in 32 bits with a bound on
@@ -24,7 +24,6 @@ namespace {
 
 constexpr float kLargest = 3.4028234663852886e38f;
 constexpr float kNone = -__builtin_huge_valf();
-constexpr uint32_t kRowsPerWave = 4;
 
 // ---- sixteen lanes -----------------------------------------------------------
 template <int CTRL>
@@ -44,9 +43,31 @@ __device__ __forceinline__ float sum16(float v) {
     v += dpp<0x122>(v);
     return v + dpp<0x121>(v);
 }
-// The lanes of the sixteen for which p holds, as bits 0 to 15.
-__device__ __forceinline__ uint32_t ballot16(bool p) {
-    return uint32_t(__ballot(p) >> (threadIdx.x & 48u)) & 0xFFFFu;
+// The same over the LANES (16 or 64) of a row: two exchanges of sixteens more.
+template <class F>
+__device__ __forceinline__ float over_wave(float v, F f) {
+    const uint32_t u = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const uint32_t w = __float_as_uint(v);
+    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+template <int LANES>
+__device__ __forceinline__ float max_row(float v) {
+    v = max16(v);
+    return LANES == 16 ? v : over_wave(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int LANES>
+__device__ __forceinline__ float sum_row(float v) {
+    v = sum16(v);
+    return LANES == 16 ? v : over_wave(v, [](float a, float b) { return a + b; });
+}
+// The row's lanes for which p holds, as bits from 0.
+template <int LANES>
+__device__ __forceinline__ uint64_t ballot_row(bool p) {
+    const uint64_t all = __ballot(p);
+    return LANES == 64 ? all : all >> (threadIdx.x & 48u) & 0xFFFFu;
 }
 // Orders a wave's own LDS accesses.
 __device__ __forceinline__ void wave_lds_sync() {
@@ -60,13 +81,16 @@ template <class T>
 struct __attribute__((packed, aligned(1))) Vec16 {
     T v[16 / sizeof(T)];
 };
-// Entries first .. first + V - 1 of a row of E, first = V times the lane of
-// sixteen, -inf beyond its end: in 16-byte pieces where the lanes share the row
-// evenly, else by way of 16 V words of LDS.
-template <int V, class T>
+// Entries first .. first + V - 1 of a row of E, first = V times the lane of the
+// row's LANES, -inf beyond its end: in 16-byte pieces where the lanes share the
+// row evenly, else one coalesced entry after the other by way of LDS, a lane's V
+// at a pitch of V + 4 for V = 16: their 16-byte reads fall into different banks.
+template <int V>
+constexpr uint32_t kGap = V >= 16 ? 4 : 0;
+template <int LANES, int V, class T>
 __device__ __forceinline__ void load_row(const T* row, uint32_t first, uint32_t E, float* staged, float* l) {
     constexpr int W = 16 / sizeof(T);
-    if (V >= W && E == 16u * V) {
+    if (V >= W && E == uint32_t(LANES) * V) {
 #pragma unroll
         for (int c = 0; c < V; c += W) {
             const Vec16<T> q = *reinterpret_cast<const Vec16<T>*>(row + first + c);
@@ -74,11 +98,14 @@ __device__ __forceinline__ void load_row(const T* row, uint32_t first, uint32_t 
             for (int j = 0; j < W && c + j < V; ++j) l[c + j] = float(q.v[j]);
         }
     } else {
-#pragma unroll 4
-        for (uint32_t e = threadIdx.x & 15u; e < 16u * V; e += 16u) staged[e] = e < E ? float(row[e]) : kNone;
+        const uint32_t c = threadIdx.x & (LANES - 1u);
+#pragma unroll
+        for (int j = 0; j < V; ++j) l[j] = c + LANES * j < E ? float(row[c + LANES * j]) : kNone;
+#pragma unroll
+        for (int j = 0; j < V; ++j) staged[c + LANES * j + (c + LANES * j) / V * kGap<V>] = l[j];
         wave_lds_sync();
 #pragma unroll
-        for (int j = 0; j < V; ++j) l[j] = staged[first + j];
+        for (int j = 0; j < V; ++j) l[j] = staged[first + first / V * kGap<V> + j];
         wave_lds_sync();
     }
 }
@@ -141,70 +168,92 @@ __device__ __forceinline__ void wave_best(double& v, uint32_t& i) {
     for (int l = 16; l < 64; l += 16) better(w, j, lane64(v, l), uint32_t(__builtin_amdgcn_readlane(int(i), l)));
     v = w, i = j;
 }
-// key: E doubles of LDS of this wave.
-template <class T>
+// A lane holds entries lane, lane + 64, ..: N of them.  Few rows come here, but a
+// launch waits for the last: its loads are in flight together and its keys in
+// registers (322 rows of 832 in bfloat16, whose groups tie now and then, with the
+// gradient: 26 us; with keys read from LDS for every choice 102).
+// key: E doubles of LDS of this wave, for the groups' ranks.
+template <int N, class T>
 __device__ __attribute__((noinline)) void choose_exact(const gf_route_opts& o, const T* row, uint32_t E, const float* bias,
                                                        double* key, int32_t* chosen) {
     const uint32_t lane = threadIdx.x & 63u;
-    double mx = kNone, z = 0.0;
-    for (uint32_t e = lane; e < E; e += 64u) mx = fmax(mx, double(entry(float(row[e]), bias, e)));
+    float l[N];
+    double mx = kNone, z = 0.0, x[N];
+    auto bias_of = [&](int n) { return bias && lane + 64u * n < E ? bias[lane + 64u * n] : 0.0f; };
+#pragma unroll
+    for (int n = 0; n < N; ++n) l[n] = lane + 64u * n < E ? float(row[lane + 64u * n]) : kNone;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {   // fmaxf takes a NaN for -inf
+        l[n] = bias_of(n) > kNone ? fminf(fmaxf(l[n], kNone), kLargest) : kNone;
+        mx = fmax(mx, double(l[n]));
+    }
     mx = wave_max(mx);
-    for (uint32_t e = lane; e < E; e += 64u) {
-        const float l = entry(float(row[e]), bias, e);
-        const double x = exp(o.score == GF_SCORE_SIGMOID ? -double(l) : double(l) - mx);
-        key[e] = l > kNone ? x : -1.0;   // a lane reads only what it wrote
-        z += l > kNone ? x : 0.0;
+    const bool sigmoid = o.score == GF_SCORE_SIGMOID;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        x[n] = exp(sigmoid ? -double(l[n]) : double(l[n]) - (mx > kNone ? mx : 0.0));
+        z += l[n] > kNone ? x[n] : 0.0;
     }
     z = wave_sum(z);
-    for (uint32_t e = lane; e < E; e += 64u) {
-        const double x = key[e], s = o.score == GF_SCORE_SIGMOID ? 1.0 / (1.0 + x) : x / z;
-        key[e] = x < 0.0 ? double(kNone) : s + (bias ? double(bias[e]) : 0.0);
-    }
-    wave_lds_sync();
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        x[n] = l[n] > kNone ? (sigmoid ? 1.0 / (1.0 + x[n]) : x[n] / z) + double(bias_of(n)) : double(kNone);
     if (o.groups > 1u) {
-        const uint32_t gs = E / o.groups;
-        double rank = kNone;
-        if (lane < o.groups) {
-            double best = kNone, second = kNone;
-#pragma unroll 4
-            for (uint32_t e = lane * gs; e < (lane + 1u) * gs; ++e) {
-                second = fmax(second, fmin(best, key[e]));
-                best = fmax(best, key[e]);
-            }
-            rank = best + (o.group_score == GF_GROUP_TOP2 && second > kNone ? second : 0.0);
-        }
-        bool kept = lane >= o.groups;
-        for (uint32_t r = 0; r < o.keep_groups; ++r) {
-            double v = kept ? double(kNone) : rank;
-            uint32_t i = kept ? ~0u : lane;
-            wave_best(v, i);
-            kept |= i == lane;
-        }
+        const uint32_t gs = E / o.groups, share = 1u << (31 - __clz(int(64u / o.groups)));   // lanes a group
+        const uint32_t g = lane / share, p = lane % share;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (lane + 64u * n < E) key[lane + 64u * n] = x[n];
         wave_lds_sync();
-        if (!kept)
-            for (uint32_t e = lane * gs; e < (lane + 1u) * gs; ++e) key[e] = kNone;
+        double best = kNone, second = kNone;
+        if (g < o.groups) {
+#pragma unroll 4
+            for (uint32_t e = p; e < gs; e += share) {
+                const double v = key[g * gs + e];
+                second = fmax(second, fmin(best, v));
+                best = fmax(best, v);
+            }
+        }
+        for (uint32_t s = 1; s < share; s <<= 1) {
+            const double u = __shfl_xor(best, int(s)), d = __shfl_xor(second, int(s));
+            second = fmax(fmax(second, d), fmin(best, u));
+            best = fmax(best, u);
+        }
+        const double rank = best + (o.group_score == GF_GROUP_TOP2 && second > kNone ? second : 0.0);
+        uint32_t place = 0;   // of the group among the ranks
+        for (uint32_t n = 0; n < o.groups; ++n) {
+            const double u = lane64(rank, int(n * share));
+            place += u > rank || (u == rank && n < g);
+        }
+        const uint64_t kept = __ballot(p == 0 && g < o.groups && place < o.keep_groups);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (!(kept >> (min(lane + 64u * n, E - 1u) / gs * share) & 1u)) x[n] = kNone;
         wave_lds_sync();
     }
     for (uint32_t r = 0; r < o.k; ++r) {
         double v = kNone;
         uint32_t i = ~0u;
-        for (uint32_t e = lane; e < E; e += 64u)
-            if (key[e] > v) v = key[e], i = e;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (x[n] > v) v = x[n], i = lane + 64u * n;
         wave_best(v, i);
-        if (lane == 0) {
-            chosen[r] = int32_t(i);   // ~0: none left
-            if (i < E) key[i] = kNone;
-        }
-        wave_lds_sync();
+        if (lane == 0) chosen[r] = int32_t(i);   // ~0: none left
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (i == lane + 64u * n) x[n] = kNone;
     }
+    wave_lds_sync();
 }
 
 // Dynamic LDS of k_route in words: the block's load counters; per wave the
 // chosen ids and the rows' keys and group ranks, or one row's keys in 64 bits.
-template <int V, uint32_t WAVES>
+template <int LANES, int V, uint32_t WAVES>
 struct RouteLds {
-    static constexpr uint32_t kKeys = 16u * V, kRow = kKeys + GF_ROUTE_MAX_GROUPS;
-    static constexpr uint32_t kWave = kRowsPerWave * (GF_ROUTE_MAX_K + kRow);
+    static constexpr uint32_t kRows = 64u / LANES;   // of a wave
+    static constexpr uint32_t kKeys = LANES * V, kRow = kKeys + std::max<uint32_t>(GF_ROUTE_MAX_GROUPS, LANES * kGap<V>);
+    static constexpr uint32_t kIds = kRows * GF_ROUTE_MAX_K;
+    static constexpr uint32_t kWave = kIds + std::max(kRows * kRow, 2u * kKeys);
     static constexpr uint32_t kBytes = 4u * (kKeys + WAVES * kWave);
 };
 
@@ -228,20 +277,29 @@ struct Three {
 // A lane holds V consecutive entries of its row: the lowest lane that has the
 // largest key has the lowest index too.  It keeps its three best at hand and
 // looks through its V again only when all are chosen and it had more: with
-// k = 8 that is once in four rows.  Groups that are whole lanes are ranked from the lanes' two
-// best, by moves between lanes; others through LDS.
-template <class T, int V, uint32_t WAVES>
-__global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_opts o, const T* logits, uint32_t rows,
-                                                                       uint32_t E, uint64_t ld, const float* bias,
-                                                                       int32_t* ids, float* weights, int32_t* load) {
+// k = 8 of 256 that is once in four rows.  Groups that are whole lanes are ranked
+// from the lanes' two best, by moves between lanes; others through LDS.
+//
+// What bounds it is the instructions issued, some 460 a row of 256, not the 1 KB
+// read: 10,000 rows of 256 in 32 bits, k = 8 by logit, take 14 us (8 us with k = 1),
+// 17 us with 4 of 16 groups kept, 22 us with the load and the launch that clears it;
+// 16,384 rows by sigmoid and bias in 8 groups 31 us.  A whole wave for a row
+// of more than 256 (8 or 16 entries a lane instead of 32 or 64, a quarter of the
+// registers) took 28 us for 4 rows of 1008 where sixteen lanes took 71, 62 for
+// 10,636 rows of 1018 where they took 73, 90 for 25,564 of 455 where they took 93.
+template <class T, int LANES, int V, uint32_t WAVES>
+__global__ __launch_bounds__(64 * WAVES, 4) void k_route(gf_route_opts o, const T* logits, uint32_t rows, uint32_t E,
+                                                         uint64_t ld, const float* bias, int32_t* ids, float* weights,
+                                                         int32_t* load) {
     extern __shared__ __align__(16) uint32_t lds[];
-    const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, mine = lane >> 4, wave = threadIdx.x >> 6;
+    using L = RouteLds<LANES, V, WAVES>;
+    constexpr uint32_t kRows = L::kRows;
+    const uint32_t lane = threadIdx.x & 63u, c = lane % LANES, mine = lane / LANES, wave = threadIdx.x >> 6;
     const uint32_t first = c * V;
-    using L = RouteLds<V, WAVES>;
     uint32_t* count = lds;
     uint32_t* own = lds + L::kKeys + wave * L::kWave;
     int32_t* chosen = reinterpret_cast<int32_t*>(own) + mine * GF_ROUTE_MAX_K;
-    float* keys = reinterpret_cast<float*>(own + kRowsPerWave * GF_ROUTE_MAX_K);
+    float* keys = reinterpret_cast<float*>(own + L::kIds);
     float *mykeys = keys + mine * L::kRow, *myranks = mykeys + L::kKeys;
     if (load) {
         for (uint32_t e = threadIdx.x; e < E; e += 64u * WAVES) count[e] = 0;
@@ -250,34 +308,34 @@ __global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_
     const bool by_score = bias || (o.groups > 1u && o.group_score == GF_GROUP_TOP2);
     const bool soft = o.score == GF_SCORE_SOFTMAX;
     // groups of whole lanes, `span` each
-    const bool whole = o.groups > 1u && E == 16u * V && 16u % o.groups == 0;
+    const bool whole = o.groups > 1u && LANES == 16 && E == 16u * V && 16u % o.groups == 0;
     const uint32_t span = whole ? 16u / o.groups : 1u;
     const uint32_t gs = E / o.groups, magic = ((1u << 20) + gs - 1u) / gs;   // e / gs = e magic >> 20 below 1024
 
-    for (uint64_t t0 = (uint64_t(blockIdx.x) * WAVES + wave) * kRowsPerWave; t0 < rows;
-         t0 += uint64_t(gridDim.x) * WAVES * kRowsPerWave) {
+    for (uint64_t t0 = (uint64_t(blockIdx.x) * WAVES + wave) * kRows; t0 < rows;
+         t0 += uint64_t(gridDim.x) * WAVES * kRows) {
         const bool row_ok = t0 + mine < rows;
         const uint64_t t = row_ok ? t0 + mine : rows - 1u;   // lanes without a row repeat the last, unstored
         const T* row = logits + t * ld;
         float key[V];
-        load_row<V>(row, first, E, mykeys, key);
+        load_row<LANES, V>(row, first, E, mykeys, key);
         float mx = kNone, top = 0.0f;   // top: the largest |bias|
         if (bias) {
             float b[V];
-            load_row<V>(bias, first, E, mykeys, b);
+            load_row<LANES, V>(bias, first, E, mykeys, b);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 key[j] = b[j] > kNone ? key[j] : kNone;
                 top = fmaxf(top, b[j] > kNone ? fabsf(b[j]) : 0.0f);
             }
-            top = max16(top);
+            top = max_row<LANES>(top);
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {   // fmaxf takes a NaN for -inf
             key[j] = fminf(fmaxf(key[j], kNone), kLargest);
             mx = fmaxf(mx, key[j]);
         }
-        mx = max16(mx);
+        mx = max_row<LANES>(mx);
         const float lift = mx > kNone ? mx : 0.0f;
         float z = 1.0f;   // of the softmax over the row
         if (soft && (by_score || !o.renormalise)) {
@@ -288,15 +346,23 @@ __global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_
                 sum += e;
                 if (by_score) key[j] = key[j] > kNone ? e : -1.0f;
             }
-            z = sum16(sum);
+            z = sum_row<LANES>(sum);
         }
-        // How far a 32-bit key k may be off: rel (|k| + top) + least.  Softmax: the
-        // difference and its product with log2 e are rounded (|difference| below
-        // 104 where the result is not 0: 2^-16 in all), and a sum of E terms is
-        // off by (V + 4) 2^-24 of itself.  Sigmoid: the error of the exponential
-        // e weighs e / (1 + e)^2 times its argument, below 1/4; the rest is a few
-        // units in the last place.
-        const float rel = soft ? 0x1p-15f : 0x1p-21f, least = soft ? 0x1p-126f : 0x1p-24f;
+        // How far a 32-bit key k may be off.  Softmax: score s = e^v / z, v <= 0.  v and
+        // its product with log2 e are rounded, so e^v is off by (2 |v| + 2) 2^-24 of
+        // itself, z by the mean of that over the scores (the mean of |v| is at most
+        // log E < 7) and (V + 6) 2^-24 for its sum, 1 / z, its product with e^v and
+        // the sum with the bias by 2^-24 each: 2^-23 s (|v| + 14 + V / 2) in all.
+        // |v| <= -log s as z >= 1, and s (c - log s) grows with s up to 1 for c >= 1: any
+        // bound of s may stand for it, |k| + top or 1.  Sigmoid: the error of
+        // e = e^-v weighs e / (1 + e)^2, below 1/4, which |v| times is below 0.23: 2^-24
+        // in all; the sum, the reciprocal (2^-23) and the sum with the bias add 2^-22 of
+        // the score and the key.
+        auto off = [&](float k) {
+            const float u = fabsf(k) + top, s = fminf(u, 1.0f);
+            return soft ? 0x1p-23f * (s * (14.0f + V / 2 - 0.6931472f * __builtin_amdgcn_logf(s + 0x1p-126f)) + u) + 0x1p-126f
+                        : 0x1p-24f + 0x1p-22f * u;
+        };
         if (by_score) {
             const float inv = 1.0f / z;
 #pragma unroll
@@ -308,22 +374,21 @@ __global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_
             }
             if (bias) {
                 float b[V];
-                load_row<V>(bias, first, E, mykeys, b);
+                load_row<LANES, V>(bias, first, E, mykeys, b);
 #pragma unroll
                 for (int j = 0; j < V; ++j) key[j] = key[j] > kNone ? key[j] + b[j] : kNone;
             }
         }
-        auto off = [&](float k) { return rel * (fabsf(k) + top) + least; };
         bool close = false;   // a comparison that 32 bits do not decide
         Three best;
         best.clear();
         auto rank_of = [&](float first_best, float second_best) {
             return first_best + (o.group_score == GF_GROUP_TOP2 && second_best > kNone ? second_best : 0.0f);
         };
-        // a rank is the sum of two keys at most; no key is below -top, so neither
-        // is beyond |rank| + top
+        // A rank is the sum of two keys at most, its rounding within their bounds; no
+        // key is below -top, so neither is beyond |rank| + top.
         auto too_close = [&](float low, float high) {
-            return by_score && high > kNone && low - high <= 2.0f * (off(low) + off(high) + 2.0f * rel * top);
+            return by_score && high > kNone && low - high <= 2.0f * (off(fabsf(low) + top) + off(fabsf(high) + top));
         };
         if (o.groups == 1u || whole) {
 #pragma unroll
@@ -346,19 +411,19 @@ __global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_
                     ahead += turn > rank || (turn == rank && (c - n & 15u) / span < c / span);
                 }
                 const bool kept = ahead < o.keep_groups * span;
-                close = too_close(-max16(kept ? -rank : kNone), max16(kept ? kNone : rank));
+                close = too_close(-max_row<LANES>(kept ? -rank : kNone), max_row<LANES>(kept ? kNone : rank));
                 if (!kept) best.clear();
             }
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) mykeys[first + j] = key[j];
             wave_lds_sync();
-            // `share` lanes a group where there are fewer than sixteen groups, or
-            // up to four groups a lane; lanes start at different places of their
-            // groups, in different banks
-            const uint32_t share = o.groups <= 2u ? 8u : o.groups <= 4u ? 4u : o.groups <= 8u ? 2u : 1u;
-            for (uint32_t i = 0; i * (16u / share) < o.groups; ++i) {
-                const uint32_t g = i * (16u / share) + c / share, p = c % share;
+            // `share` lanes a group, or up to four groups a lane; lanes start at
+            // different places of their groups, in different banks
+            const uint32_t wide = o.groups < uint32_t(LANES) ? 31u - uint32_t(__clz(int(LANES / o.groups))) : 0u;
+            const uint32_t share = 1u << wide, p = c % share;
+            for (uint32_t i = 0; i < o.groups; i += LANES >> wide) {
+                const uint32_t g = i + (c >> wide);
                 float u = kNone, d = kNone;
                 if (g < o.groups && p < gs) {
                     const uint32_t n = (gs - p + share - 1u) / share;   // entries p, p + share, ..
@@ -382,7 +447,7 @@ __global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_
             // a group's place among the ranks; kept are the first keep_groups
             uint64_t kept = 0;
             float low = -kNone, high = kNone;   // the last kept rank, the first not kept
-            for (uint32_t i = 0; i < o.groups; i += 16u) {
+            for (uint32_t i = 0; i < o.groups; i += LANES) {
                 const uint32_t g = i + c;
                 const float v = g < o.groups ? myranks[g] : kNone;
                 uint32_t place = 0;
@@ -392,11 +457,11 @@ __global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_
                     place += u > v || (u == v && n < g);
                 }
                 const bool in = g < o.groups && place < o.keep_groups;
-                kept |= uint64_t(ballot16(in)) << i;
+                kept |= ballot_row<LANES>(in) << i;
                 if (in) low = fminf(low, v);
                 else if (g < o.groups) high = fmaxf(high, v);
             }
-            close = too_close(-max16(-low), max16(high));
+            close = too_close(-max_row<LANES>(-low), max_row<LANES>(high));
             // the entries' groups, counted up; not ahead of the loop over rows, which
             // would take a register each
             uint32_t g = first * magic >> 20, left = (g + 1u) * gs - first;
@@ -413,13 +478,22 @@ __global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_
         float before = 0.0f;
         bool more = best.v[2] > kNone;   // the lane may have a fourth
         for (uint32_t n = 0; n <= o.k; ++n) {
-            const float m = max16(best.v[0]);
-            if (by_score && n && m > kNone) close |= before - m <= off(before) + off(m);
+            const float m = max_row<LANES>(best.v[0]);
+            const uint64_t who = ballot_row<LANES>(best.v[0] == m && m > kNone);
+            if (by_score && n) {
+                bool near = who && before - m <= off(before) + off(m);
+                if (__any(near)) {   // the same logit and bias: an exact tie, the lower index first
+                    wave_lds_sync();
+                    const uint32_t at = __shfl(best.i[0], int(mine * LANES + (who ? uint32_t(__ffsll((long long)who)) - 1u : 0u)));
+                    const uint32_t last = near ? uint32_t(chosen[n - 1u]) : 0u;
+                    if (near && row[at] == row[last] && (!bias || bias[at] == bias[last])) near = false;
+                }
+                close |= near;
+            }
             before = m;
             if (n == o.k) break;
-            const uint32_t who = ballot16(best.v[0] == m && m > kNone);
             if (!who && c == 0) chosen[n] = -1;
-            if (who && c == uint32_t(__ffs(int(who))) - 1u) {
+            if (who && c == uint32_t(__ffsll((long long)who)) - 1u) {
                 const uint32_t last = best.i[0];
                 chosen[n] = int32_t(last);
                 best.v[0] = best.v[1], best.i[0] = best.i[1];
@@ -438,32 +512,32 @@ __global__ __launch_bounds__(64 * WAVES, V >= 32 ? 2 : 4) void k_route(gf_route_
         if (by_score) {
             uint64_t again = __ballot(close && c == 0);
             while (again) {
-                const uint32_t r = uint32_t(__ffsll((long long)again) - 1) / 16u;
+                const uint32_t r = uint32_t(__ffsll((long long)again) - 1) / LANES;
                 again &= again - 1u;
-                choose_exact(o, logits + min(t0 + r, uint64_t(rows) - 1u) * ld, E, bias, reinterpret_cast<double*>(keys),
+                choose_exact<(LANES * V + 63) / 64>(o, logits + min(t0 + r, uint64_t(rows) - 1u) * ld, E, bias, reinterpret_cast<double*>(keys),
                              reinterpret_cast<int32_t*>(own) + r * GF_ROUTE_MAX_K);
             }
         }
-        // up to four of the row's choices a lane
-        float s[4], l[4], sum = 0.0f, peak = kNone;
-        int32_t id[4];
+        constexpr uint32_t kChoices = GF_ROUTE_MAX_K / LANES;   // of the row, a lane, at most
+        float s[kChoices], l[kChoices], sum = 0.0f, peak = kNone;
+        int32_t id[kChoices];
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            const uint32_t n = i * 16u + c;
+        for (uint32_t i = 0; i < kChoices; ++i) {
+            const uint32_t n = i * LANES + c;
             id[i] = n < o.k ? chosen[n] : -1;
             l[i] = id[i] >= 0 ? fminf(float(row[id[i]]), kLargest) : kNone;
             peak = fmaxf(peak, l[i]);
         }
-        if (o.renormalise) mx = max16(peak);   // the softmax over the row cancels
+        if (o.renormalise) mx = max_row<LANES>(peak);   // the softmax over the row cancels
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
+        for (uint32_t i = 0; i < kChoices; ++i) {
             s[i] = id[i] < 0 ? 0.0f : soft ? expf(l[i] - mx) / (o.renormalise ? 1.0f : z) : sigmoid(l[i]);
             sum += s[i];
         }
-        if (o.renormalise) sum = sum16(sum);
+        if (o.renormalise) sum = sum_row<LANES>(sum);
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            const uint32_t n = i * 16u + c;
+        for (uint32_t i = 0; i < kChoices; ++i) {
+            const uint32_t n = i * LANES + c;
             if (!row_ok || n >= o.k) continue;
             ids[t * o.k + n] = id[i];
             weights[t * o.k + n] = o.scale * (o.renormalise ? sum > 0.0f ? s[i] / sum : 0.0f : s[i]);
@@ -486,7 +560,7 @@ __global__ void k_route_clear(int32_t* load, uint32_t E) {
 // The gradient, sixteen lanes a row as above: the k chosen entries' terms are
 // put into a row of LDS that is written out whole; the softmax over all
 // entries adds its term to every live one.
-constexpr uint32_t kGradWaves = 4;
+constexpr uint32_t kGradWaves = 4, kGradRows = 4;   // a block's waves, a wave's rows
 template <class T>
 __global__ __launch_bounds__(64 * kGradWaves) void k_route_grad(gf_route_opts o, const T* logits, uint32_t rows, uint32_t E,
                                                             uint64_t ld, const float* bias, const int32_t* ids,
@@ -494,14 +568,13 @@ __global__ __launch_bounds__(64 * kGradWaves) void k_route_grad(gf_route_opts o,
     extern __shared__ __align__(16) uint32_t lds[];
     const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, wave = threadIdx.x >> 6;
     const uint32_t pitch = E + 7u & ~7u;
-    float* d = reinterpret_cast<float*>(lds) + (wave * kRowsPerWave + (lane >> 4)) * pitch;
+    float* d = reinterpret_cast<float*>(lds) + (wave * kGradRows + (lane >> 4)) * pitch;
     const bool soft = o.score == GF_SCORE_SOFTMAX;
-    for (uint64_t t0 = (uint64_t(blockIdx.x) * kGradWaves + wave) * kRowsPerWave; t0 < rows;
-         t0 += uint64_t(gridDim.x) * kGradWaves * kRowsPerWave) {
+    for (uint64_t t0 = (uint64_t(blockIdx.x) * kGradWaves + wave) * kGradRows; t0 < rows;
+         t0 += uint64_t(gridDim.x) * kGradWaves * kGradRows) {
         const bool row_ok = t0 + (lane >> 4) < rows;
         const uint64_t t = row_ok ? t0 + (lane >> 4) : rows - 1u;
         const T* row = logits + t * ld;
-        for (uint32_t e = c * 4u; e < pitch; e += 64u) *reinterpret_cast<float4*>(d + e) = make_float4(0, 0, 0, 0);
         float l[4], g[4], s[4], sum = 0.0f, peak = kNone, mx = kNone, z = 0.0f;
         int32_t id[4];
 #pragma unroll
@@ -516,11 +589,17 @@ __global__ __launch_bounds__(64 * kGradWaves) void k_route_grad(gf_route_opts o,
         }
         const bool all = soft && !o.renormalise;
         if (all) {
-            for (uint32_t e = c; e < E; e += 16u) mx = fmaxf(mx, entry(float(row[e]), bias, e));
-            mx = max16(mx);
+#pragma unroll 4
             for (uint32_t e = c; e < E; e += 16u) {
-                const float v = entry(float(row[e]), bias, e);
-                if (v > kNone) z += expf(v - mx);
+                d[e] = entry(float(row[e]), bias, e);
+                mx = fmaxf(mx, d[e]);
+            }
+            mx = max16(mx);
+            const float lift = mx > kNone ? mx : 0.0f;
+#pragma unroll 4
+            for (uint32_t e = c; e < E; e += 16u) {   // a lane reads only what it wrote
+                d[e] = expf(d[e] - lift);             // 0 for a masked entry
+                z += d[e];
             }
             z = sum16(z);
         } else {
@@ -549,18 +628,20 @@ __global__ __launch_bounds__(64 * kGradWaves) void k_route_grad(gf_route_opts o,
 #pragma unroll
             for (uint32_t i = 0; i < 4u; ++i) g[i] *= o.scale * s[i] * (1.0f - s[i]);
         }
+        if (all) {
+            const float w = z > 0.0f ? -o.scale * mean / z : 0.0f;
+#pragma unroll 4
+            for (uint32_t e = c; e < E; e += 16u) d[e] = d[e] > 0.0f ? d[e] * w : 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) g[i] = o.scale * s[i] * (g[i] - mean);
+        } else {
+            for (uint32_t e = c * 4u; e < pitch; e += 64u) *reinterpret_cast<float4*>(d + e) = make_float4(0, 0, 0, 0);
+        }
         wave_lds_sync();
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i)
             if (id[i] >= 0) d[id[i]] = g[i];
         wave_lds_sync();
-        if (all) {
-            for (uint32_t e = c; e < E; e += 16u) {
-                const float v = entry(float(row[e]), bias, e);
-                d[e] = v > kNone ? o.scale * (expf(v - mx) / z) * (d[e] - mean) : 0.0f;
-            }
-            wave_lds_sync();
-        }
         if (row_ok) {
             constexpr uint32_t W = 16 / sizeof(T);
             T* out = dlogits + t * ldd;
@@ -584,46 +665,50 @@ hipError_t by_type(int32_t dtype, F&& f) {
     if (dtype == GF_F16) return f(_Float16());
     return f(__bf16());
 }
+// f(lanes a row, entries a lane)
 template <class F>
 hipError_t by_width(uint32_t E, F&& f) {
-    if (E <= 16u) return f(std::integral_constant<int, 1>());
-    if (E <= 32u) return f(std::integral_constant<int, 2>());
-    if (E <= 64u) return f(std::integral_constant<int, 4>());
-    if (E <= 128u) return f(std::integral_constant<int, 8>());
-    if (E <= 256u) return f(std::integral_constant<int, 16>());
-    if (E <= 512u) return f(std::integral_constant<int, 32>());
-    return f(std::integral_constant<int, 64>());
+    constexpr std::integral_constant<int, 16> kPart;
+    constexpr std::integral_constant<int, 64> kWave;
+    if (E <= 16u) return f(kPart, std::integral_constant<int, 1>());
+    if (E <= 32u) return f(kPart, std::integral_constant<int, 2>());
+    if (E <= 64u) return f(kPart, std::integral_constant<int, 4>());
+    if (E <= 128u) return f(kPart, std::integral_constant<int, 8>());
+    if (E <= 256u) return f(kPart, std::integral_constant<int, 16>());
+    if (E <= 512u) return f(kWave, std::integral_constant<int, 8>());
+    return f(kWave, std::integral_constant<int, 16>());
 }
-// A wave has four rows at a time; beyond this many blocks it takes more.
-uint32_t route_blocks(uint64_t rows, uint32_t waves) {
-    return uint32_t(std::min<uint64_t>((rows + waves * kRowsPerWave - 1u) / (waves * kRowsPerWave), 8192u / waves));
+// Beyond this many blocks a wave takes more than its first rows.
+uint32_t route_blocks(uint64_t rows, uint32_t waves, uint32_t rows_of_wave) {
+    return uint32_t(std::min<uint64_t>((rows + waves * rows_of_wave - 1u) / (waves * rows_of_wave), 8192u / waves));
 }
 
 }  // namespace
 
-hipError_t launch_route(const gf_route_opts& o, const MatIn& logits, uint32_t E, const float* bias, int32_t* ids,
+hipError_t launch_route(const gf_route_opts& opts, const MatIn& logits, uint32_t E, const float* bias, int32_t* ids,
                         float* weights, int32_t* load, hipStream_t st) {
     if (load) {
         hipLaunchKernelGGL(k_route_clear, dim3((E + 255u) / 256u), 256, 0, st, load, E);
         if (const hipError_t e = hipGetLastError()) return e;
     }
     if (!logits.rows) return hipSuccess;
+    gf_route_opts o = opts;
+    if (o.keep_groups == o.groups) o.groups = o.keep_groups = 1;   // all groups: the same as none
     return by_type(logits.dtype, [&](auto v) {
-        return by_width(E, [&](auto width) {
+        return by_width(E, [&](auto lanes, auto width) {
             using T = decltype(v);
-            constexpr int V = decltype(width)::value;
+            constexpr int kLanes = decltype(lanes)::value, V = decltype(width)::value;
             auto go = [&](auto waves) {
                 constexpr uint32_t W = decltype(waves)::value;
-                constexpr uint32_t kLds = RouteLds<V, W>::kBytes;
-                hipLaunchKernelGGL((k_route<T, V, W>), dim3(route_blocks(logits.rows, W)), 64 * W, kLds, st, o,
-                                   static_cast<const T*>(logits.p), uint32_t(logits.rows), E, logits.ld, bias, ids, weights,
-                                   load);
+                using L = RouteLds<kLanes, V, W>;
+                hipLaunchKernelGGL((k_route<T, kLanes, V, W>), dim3(route_blocks(logits.rows, W, L::kRows)), 64 * W,
+                                   L::kBytes, st, o, static_cast<const T*>(logits.p), uint32_t(logits.rows), E, logits.ld,
+                                   bias, ids, weights, load);
                 return hipGetLastError();
             };
             // a block ends with an atomic addition for every entry that it counted:
             // where rows fill the chip anyway, few large blocks
-            if constexpr (V <= 16)
-                if (load && logits.rows >= 8192u) return go(std::integral_constant<uint32_t, 16>());
+            if (load && logits.rows >= 8192u) return go(std::integral_constant<uint32_t, 16>());
             return go(std::integral_constant<uint32_t, 4>());
         });
     });
@@ -633,8 +718,8 @@ hipError_t launch_route_grad(const gf_route_opts& o, const MatIn& logits, uint32
                              const int32_t* ids, const float* dweights, const MatOut& dlogits, hipStream_t st) {
     return by_type(logits.dtype, [&](auto v) {
         using T = decltype(v);
-        hipLaunchKernelGGL(k_route_grad<T>, dim3(route_blocks(logits.rows, kGradWaves)), 64 * kGradWaves,
-                           kGradWaves * kRowsPerWave * (E + 7u & ~7u) * 4u, st, o, static_cast<const T*>(logits.p),
+        hipLaunchKernelGGL(k_route_grad<T>, dim3(route_blocks(logits.rows, kGradWaves, kGradRows)), 64 * kGradWaves,
+                           kGradWaves * kGradRows * (E + 7u & ~7u) * 4u, st, o, static_cast<const T*>(logits.p),
                            uint32_t(logits.rows), E, logits.ld, bias, ids, dweights, static_cast<T*>(dlogits.p), dlogits.ld);
         return hipGetLastError();
     });

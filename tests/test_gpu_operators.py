@@ -384,6 +384,27 @@ def test_route_ties_and_near_ties(score):
         assert np.array_equal(_np(got.ids), ids)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,keep,k", [(12, 4, 2, 5), (120, 8, 8, 30), (256, 16, 4, 8), (300, 1, 1, 64), (320, 10, 4, 9),
+                                             (512, 64, 20, 16), (1000, 8, 3, 12), (1024, 1, 1, 1)])
+def test_route_ties_of_rounded_logits(E, groups, keep, k, score):
+    """Logits of few values: equal sums of score and bias, equal ranks of groups,
+    in rows of every width; bias none, nothing, or of few values."""
+    _case("rounded", E, groups, keep, k, score)
+    g = torch.Generator().manual_seed(E + k)
+    l = (2 * torch.randn(150, E, generator=g)).to(torch.bfloat16)
+    l[1::2] = torch.round(l[1::2] * 2) / 2
+    l[7::10, E // 3:] = float("-inf")
+    for bias in (None, torch.zeros(E), torch.randint(-1, 2, (E,), generator=g) / 16):
+        for rank in ("max", "top2"):
+            got = gf.route(l.cuda(), k, bias=None if bias is None else bias.cuda(), score=score, groups=groups,
+                           keep_groups=keep, group_score=rank)
+            ids, w, load = orc.route(_np(l), k, bias=None if bias is None else bias.double().numpy(), score=score,
+                                     groups=groups, keep_groups=keep, group_score=rank)
+            assert np.array_equal(_np(got.ids), ids) and np.array_equal(_np(got.load), load)
+            _close(got.weights, w, orc.WEIGHT_RTOL * np.abs(w) + 2.0 ** -126, "weights")
+
+
 def test_route_grad_ignores_foreign_ids():
     _case("foreign ids")
     l = _rows(4, 16, torch.float32, 1, spread=False)
