@@ -148,10 +148,9 @@ inline uint32_t compute_units() {
 // Whether a result of M x N is better cut into tiles of 256 than of 128.  A
 // compute unit holds one of the large or two of the small ones, and a large one
 // takes as long as two rounds of small ones at most: so where it does not take
-// more rounds.  Large against small, at four bits: 8192 x 8192 x 4096 187 us
+// more rounds.  Large against small: 8192 x 8192 x 4096 187 us
 // against 250, 4096 x 4096 x 2048 26 against 30, 1000 x 4096 x 4096 32 against
-// 18, 1000 x 20000 x 768 23 against 20; in bfloat16: 4096 x 4096 x 2048 69
-// against 86, 2048 x 4096 x 4096 107 against 89, 1000 x 20000 x 768 50 against 45.
+// 18, 1000 x 20000 x 768 23 against 20.
 inline bool large_tiles(uint64_t M, uint64_t N, uint64_t cus) {
     const uint64_t big = ((M + 255u) / 256u) * ((N + 255u) / 256u), small = ((M + 127u) / 128u) * ((N + 127u) / 128u);
     return 2u * ((big + cus - 1u) / cus) <= (small + 2u * cus - 1u) / (2u * cus);

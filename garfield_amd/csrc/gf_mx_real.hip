@@ -198,9 +198,10 @@ __global__ __launch_bounds__(64 * WK) void k_mx_few(const ElemT<DT>* x, uint32_t
 // comes through registers, one block of 32 values a thread, decoded on its way
 // to LDS, loaded one step ahead (two slots).  A real side in bfloat16 (or in
 // planes, one after the other) comes by copies straight to LDS, two steps ahead
-// (three slots); one in binary16 or fp32 through registers, split into its
-// planes on its way, one step ahead (two slots): a small result is then one
-// launch, and the planes share what is read and decoded of the other side.  A
+// (three slots; COPIED); one in binary16 or fp32, or whose rows are not whole
+// steps, through registers, split into its planes on its way, one step ahead (two
+// slots): a small result is then one launch, and the planes share what is read
+// and decoded of the other side.  A
 // step has four parts; a part's operands are read from LDS while the part before
 // it is multiplied, across steps too.
 // Columns are rows of w (TR = false: the product) or positions in w's rows
@@ -215,10 +216,10 @@ __global__ __launch_bounds__(64 * WK) void k_mx_few(const ElemT<DT>* x, uint32_t
 // The sum may be cut into `parts`, each block then writing its own in fp32 to
 // a workspace (out, rows of ldo, a part every M ldo), which k_mx_join adds up
 // in order.
-template <int DT, int BM, int BN, int OT, bool TR>
+template <int DT, bool COPIED, int BM, int BN, int OT, bool TR>
 struct RealLds {
-    static constexpr bool kSplit = DT != GF_BF16;
-    static constexpr uint32_t kPlane = BM * 128u, kA = kPlane * kPlanes<DT>, kB = BN * 128u, kSlots = kSplit ? 2u : 3u;
+    static_assert(DT == GF_BF16 || !COPIED, "");
+    static constexpr uint32_t kPlane = BM * 128u, kA = kPlane * kPlanes<DT>, kB = BN * 128u, kSlots = COPIED ? 3u : 2u;
     static constexpr uint32_t kBytes = kSlots * kA + 2u * kB;
     static constexpr uint32_t kCols = 32u;
     using P = Piece<OT, kCols>;
@@ -234,9 +235,9 @@ struct RealArgs {
     uint32_t tm, tn, parts;
 };
 
-template <int DT, int BM, int BN, int VM, int VN, int OT, bool TR>
+template <int DT, bool COPIED, int BM, int BN, int VM, int VN, int OT, bool TR>
 __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>* out, uint64_t ldo) {
-    using L = RealLds<DT, BM, BN, OT, TR>;
+    using L = RealLds<DT, COPIED, BM, BN, OT, TR>;
     using Pc = typename L::P;
     constexpr int P = kPlanes<DT>;
     constexpr uint32_t TH = 64u * VM * VN, kPer = BM * 8u / TH;   // 8-value pieces of the real side a thread and step
@@ -257,21 +258,21 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
     // The thread's pieces: row i (TH / 8) + tid / 8, place tid & 7.  Rows beyond
     // the end repeat the last one; their sums are not stored.
     const uint32_t piece_of = (tid & 7u) ^ (tid >> 4 & 7u);
-    uint32_t oa[kPer];                                   // bfloat16: byte offsets for the copies
-    const ElemT<DT>* ra[kPer];                           // else the rows,
+    uint32_t oa[kPer];                                   // byte offsets for the copies,
+    const ElemT<DT>* ra[kPer];                           // or the rows
     constexpr uint32_t kRaw = sizeof(ElemT<DT>) / 2u;    // and eight values of each as loaded
     uint4 raw[kPer][kRaw];
     const uint8_t* pa = static_cast<const uint8_t*>(p.a) + uint64_t(m0) * p.lda * 2u;
 #pragma unroll
     for (uint32_t i = 0; i < kPer; ++i) {
         const uint32_t row = min(i * (TH / 8u) + tid / 8u, p.M - 1u - m0);
-        if constexpr (L::kSplit)
+        if constexpr (!COPIED)
             ra[i] = static_cast<const ElemT<DT>*>(p.a) + uint64_t(m0 + row) * p.lda;
         else
             oa[i] = row * uint32_t(p.lda * 2u) + piece_of * 16u;
     }
     auto load_a = [&](uint32_t s, uint32_t slot) {
-        if constexpr (!L::kSplit) {
+        if constexpr (COPIED) {
             const uint8_t* at = pa + uint64_t(s) * p.step * 2u;
 #pragma unroll
             for (uint32_t i = 0; i < kPer; ++i) lds_copy16(at, oa[i], base + slot * L::kA + i * TH * 16u + wave * 1024u);
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
         }
     };
     auto write_a = [&](uint32_t slot) {
-        if constexpr (L::kSplit) {
+        if constexpr (!COPIED) {
 #pragma unroll
             for (uint32_t i = 0; i < kPer; ++i) {
                 ElemT<DT> e[8];
@@ -421,12 +422,12 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
         const uint32_t next = min(s0 + 1u, s1 - 1u);
         load_a(s0, 0);
         load_b(s0);
-        if constexpr (!L::kSplit) load_a(next, 1);
+        if constexpr (COPIED) load_a(next, 1);
         uint4 raw0[kPer][kRaw];
         __builtin_memcpy(raw0, raw, sizeof(raw));
         const uint4 code0 = code;
         const uint32_t byte0 = byte;
-        if constexpr (L::kSplit) load_a(next, 1);
+        if constexpr (!COPIED) load_a(next, 1);
         load_b(next);
         wait_vmcnt<0>();
         write_a(1);
@@ -490,33 +491,63 @@ __global__ __launch_bounds__(256) void k_mx_zero(uint64_t M, uint32_t N, ElemT<O
 
 uint32_t blocks_for(uint64_t items) { return uint32_t(std::min<uint64_t>((items + 255u) / 256u, 1u << 20)); }
 
-// How a product of M real rows of J values with N columns runs: the tile, and
-// the sum in parts where the tiles leave compute units idle (at least four
-// steps of 64 a part, one part a compute unit, and no more partial sums than 64
-// MiB).  The plan is part of the interface (the workspace's size), so it is made
-// for the chip's compute units, not the current device's.
+// How a product of M real rows of J values with N columns runs: the tile, the
+// real side as planes or split in the kernel, and the sum in parts where the
+// tiles leave compute units idle (at least four steps of 64 a part, and no more
+// partial sums than 64 MiB).  The plan is part of the interface (the workspace's
+// size), so it is made for the chip's compute units, not the current device's.
 constexpr uint64_t kUnits = 256;
+enum Tile { kLarge, kSmall, kSplit };
 struct RealPlan {
-    bool large, planes;   // tiles of 256; the real side as planes in the workspace
+    Tile tile;
+    bool planes;   // the real side as planes in the workspace
     uint32_t tm, tn, parts;
 };
-RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
-    RealPlan r;
-    r.large = large_tiles(M, N, kUnits);
-    // Binary16 and fp32 pay for planes only where tiles are large.  fp32, planes
-    // against splitting in the kernel: 4096 x 8192 x 4096 735 us against 1008,
-    // 2048 x 4096 x 4096 268 against 292, 2048 x 2048 x 4096 169 against 151, the
-    // gradient of 500 queries over 60000 rows of 128 107 against 47.
-    r.planes = dtype == GF_BF16 || r.large;
-    const uint64_t tm = r.large ? 256u : r.planes ? 128u : 64u, tn = r.large ? 256u : 128u;
-    r.tm = uint32_t((M + tm - 1u) / tm), r.tn = uint32_t((N + tn - 1u) / tn);
-    // two of the smaller tiles share a compute unit
-    uint64_t parts = std::min<uint64_t>((r.planes ? 1u : 2u) * kUnits / (uint64_t(r.tm) * r.tn), (J + 63u) / 64u / 4u);
-    parts = std::min<uint64_t>(parts, (16u << 20) / (M * N));
-    r.parts = uint32_t(std::max<uint64_t>(parts, 1u));
-    return r;
-}
 uint32_t planes_of(int32_t dtype) { return dtype == GF_BF16 ? 1u : dtype == GF_F16 ? 2u : 3u; }
+// The plan is the tile whose time, in us, is the least by this account: rounds of
+// the chip's tiles, for each a step's time (one tile on a compute unit; two of
+// the smaller ones) and once what a tile takes besides; a launch and 7 TB/s for
+// planes and for joining parts, which are read back from the caches for the most
+// part.  Fitted to 168 products and gradients of 17 to 10,000 real rows with each
+// tile: nine in ten of its times are within 15% of the measured one, and the
+// tile it takes was 1% slower than the best on average and 18% at most.  Large,
+// small, split: fp32, 4096 x 8192 x 4096 721, 867, 935 us, 2048 x 2048 x 4096 120,
+// 148, 135; binary16, 1024 x 53124 x 1024 212, 223, 328, the gradient of 777
+// queries over 9376 rows of 100 38, 27, 20, in bfloat16 31, 23, 18; bfloat16, 4096 x
+// 8192 x 4096 217, 282, 2048 x 2048 x 4096 57, 45.
+struct TileCost {
+    float one, two, besides;
+};
+constexpr TileCost kTileCost[3][3] = {   // by tile, by type (GF_F32, GF_F16, GF_BF16)
+    {{1.75f, 1.75f, 6.0f}, {1.51f, 1.51f, 6.0f}, {1.62f, 1.62f, 6.0f}},
+    {{0.72f, 1.06f, 2.2f}, {0.65f, 1.00f, 2.2f}, {0.67f, 1.06f, 2.2f}},
+    {{1.16f, 2.02f, 2.2f}, {0.99f, 1.60f, 2.0f}, {0.80f, 1.25f, 1.2f}}};
+constexpr float kLaunch = 3.0f, kByte = 1.0f / 7e6f;
+RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
+    RealPlan best = {};
+    float least = 0.0f;
+    const uint64_t steps = (J + 63u) / 64u;
+    const bool in_steps = dtype == GF_BF16 && J % 64u == 0;   // read in place where aligned
+    for (const Tile tile : {kLarge, kSmall, kSplit}) {
+        if (tile == kSplit && in_steps) continue;
+        const uint64_t bm = tile == kLarge ? 256u : tile == kSmall ? 128u : 64u, bn = tile == kLarge ? 256u : 128u;
+        const uint64_t tm = (M + bm - 1u) / bm, tn = (N + bn - 1u) / bn, planes = tile == kSplit ? 1u : planes_of(dtype);
+        uint64_t parts = std::min<uint64_t>((tile == kSplit ? 2u : 1u) * kUnits / (tm * tn), steps / 4u);
+        parts = std::max<uint64_t>(std::min<uint64_t>(parts, (16u << 20) / (M * N)), 1u);
+        const TileCost& c = kTileCost[tile][dtype];
+        const uint64_t tiles = tm * tn * parts, round = tile == kLarge ? kUnits : 2u * kUnits;
+        const uint64_t full = tiles / round, rest = tiles % round;
+        const float step = float(full) * c.two + (rest == 0 ? 0.0f : rest <= kUnits ? c.one : c.two);
+        float us = step * float((steps * planes + parts - 1u) / parts) + c.besides * float(full + (rest != 0));
+        if (tile != kSplit && !in_steps)
+            us += kLaunch + float(M) * float(J) * float(dtype == GF_F32 ? 10 : dtype == GF_F16 ? 6 : 4) * kByte;
+        if (parts > 1u) us += kLaunch + float(M) * float(N) * float(parts) * 8.0f * kByte;
+        if (best.tm && us >= least) continue;
+        least = us;
+        best = {tile, tile != kSplit, uint32_t(tm), uint32_t(tn), uint32_t(parts)};
+    }
+    return best;
+}
 // Whether a bfloat16 side can be read in place: rows of whole steps, aligned
 // for the copies.
 bool in_place(const MatIn& a, uint64_t J) {
@@ -547,14 +578,16 @@ hipError_t real_product(const MatIn& a, uint64_t J, const gf_mx_rows& w, uint64_
         constexpr int OT = decltype(ot)::value;
         ElemT<OT>* o = static_cast<ElemT<OT>*>(to);
         const dim3 grid(pl.tm * pl.tn * pl.parts);
-        if (pl.large)
-            hipLaunchKernelGGL((k_mx_real<GF_BF16, 256, 256, 2, 4, OT, TR>), grid, 512, 0, st, p, o, ldo);
+        if (pl.tile == kLarge)
+            hipLaunchKernelGGL((k_mx_real<GF_BF16, true, 256, 256, 2, 4, OT, TR>), grid, 512, 0, st, p, o, ldo);
+        else if (pl.tile == kSmall)
+            hipLaunchKernelGGL((k_mx_real<GF_BF16, true, 128, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
         else if (a.dtype == GF_BF16)
-            hipLaunchKernelGGL((k_mx_real<GF_BF16, 128, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
+            hipLaunchKernelGGL((k_mx_real<GF_BF16, false, 64, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
         else if (a.dtype == GF_F16)
-            hipLaunchKernelGGL((k_mx_real<GF_F16, 64, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
+            hipLaunchKernelGGL((k_mx_real<GF_F16, false, 64, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
         else
-            hipLaunchKernelGGL((k_mx_real<GF_F32, 64, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
+            hipLaunchKernelGGL((k_mx_real<GF_F32, false, 64, 128, 2, 2, OT, TR>), grid, 256, 0, st, p, o, ldo);
         return hipGetLastError();
     };
     if (pl.parts == 1u) return by_type(out.dtype, [&](auto ot) { return run(ot, out.p, out.ld); });
