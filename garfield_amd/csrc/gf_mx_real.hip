@@ -618,15 +618,29 @@ hipError_t launch_mx_product(const MatIn& x, const gf_mx_rows& w, const MatOut& 
                                    static_cast<ElemT<OT>*>(out.p), out.ld);
                 return hipGetLastError();
             };
-            // Many queries share each decoded block, few are bound by the loads of
-            // codes, and few rows leave compute units idle.  Rows of 4096, 16384
-            // of them: 16 queries 13.7 us by <4, 8> against 15.2 by <2, 4>, one
-            // query 12.0 against 9.8; one query, 4096 rows of 1024: 4.3 us by <2, 4>
-            // against 3.3 by <1, 8>.
-            if (S >= 8 && x.rows > 4) return go(std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
-            if (S >= 8 && w.rows >= 8192) return go(std::integral_constant<int, 2>(), std::integral_constant<int, 4>());
-            if (S >= 8) return go(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
-            return go(std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
+            // Waves that fill the chip need not share K; where rows are few, they do.
+            // A real side that is split takes more of a wave's time than the decoding,
+            // so a split goes with more rows.  One query, <1, 1>, <2, 1>, <2, 4>, <1, 8>:
+            // bfloat16, 53124 rows of 1024 8.3, 8.1, 13.6, 15.2 us, 16384 of 4096 14.2, 17.6,
+            // 9.5, 10.6, 2000 of 8000 26, 33, 12, 8; binary16, <1, 1>, <4, 1>, <4, 4>, <4, 8>,
+            // <2, 8>, <1, 8>: 300000 of 100 21, 12, 20, 41, 58, 101; 200000 of 2000 153, 99,
+            // 76, 93, 115, 188; 16384 of 4096 35, 48, 18, 16, 18, 26; 8192 of 4096 31, 46, 17,
+            // 15, 12, 15; 2000 of 8000 63, 94, 32, 25, 21, 18.
+            const std::integral_constant<int, 1> one;
+            const std::integral_constant<int, 2> two;
+            const std::integral_constant<int, 4> four;
+            const std::integral_constant<int, 8> eight;
+            if constexpr (DT == GF_BF16) {
+                if (w.rows >= 49152) return go(two, one);
+                if (S >= 8 && w.rows >= 8192) return go(two, four);
+            } else {
+                if (w.rows >= 49152 && S <= 4) return go(four, one);
+                if (w.rows >= 49152 || (w.rows >= 12288 && S >= 4 && S < 8)) return go(four, four);
+                if (S >= 8 && w.rows >= 12288) return go(four, eight);
+                if (S >= 8 && w.rows >= 4096) return go(two, eight);
+            }
+            if (S >= 8) return go(one, eight);
+            return go(one, one);
         });
     });
 }

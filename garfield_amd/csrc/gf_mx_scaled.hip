@@ -329,12 +329,30 @@ hipError_t tile(const gf_mx_rows& x, const gf_mx_rows& w, const MatOut& out, hip
 hipError_t launch_mx_product_mx(const gf_mx_rows& x, const gf_mx_rows& w, const MatOut& out, void*, hipStream_t st) {
     const uint64_t M = x.rows, N = w.rows;
     const uint32_t S = mx_chunks(w.K);
+    // Up to 16 queries: loads straight to registers, but many long rows come faster
+    // by copies: direct against tiles, 16 x 53124 x 1024 14.5 us against 9.4, 5 x
+    // 200000 x 2000 63 against 41; 16 x 16384 x 4096 11 against 15, 16 x 300000 x 640 29
+    // against 32.
+    if (M <= 16 && S >= 8 && N >= 32768 && S < 1u << 18) return tile<128, 128, 2, 2>(x, w, out, st);
     if (M <= 16) return S >= 8 ? direct<1, 1, 1, 8>(x, w, out, st) : direct<1, 1, 1, 1>(x, w, out, st);
     if (S >= 4 && S < 1u << 18) {
         if (large_tiles(M, N, compute_units())) return tile<256, 256, 2, 4>(x, w, out, st);
-        if (((M + 127) / 128) * ((N + 127) / 128) >= 128) return tile<128, 128, 2, 2>(x, w, out, st);
+        // The tile of the least time by this account, in us: what a launch takes
+        // besides, and for every chunk of K that of the blocks on a compute unit.
+        // 32 x 32, 16 x 16, 32 x 64 and 128 x 128 measured: 17 x 2048 x 8192 14, 9, 23,
+        // 26; 128 x 2048 x 8192 17, 30, 25, 25; 512 x 2048 x 8192 59, 114, 46, 25; 32 x
+        // 53124 x 1024 19, 27, 14, 9; 26 x 1931 x 3352 6, 4, 9, 14; 500 x 500 x 1500 5, 7,
+        // 7, 10.
+        auto us = [&](uint64_t bm, uint64_t bn, float besides, float chunk) {
+            const uint64_t blocks = ((M + bm - 1u) / bm) * ((N + bn - 1u) / bn);
+            return besides + chunk * float(S) * std::max(1.0f, float(blocks) / 256.0f);
+        };
+        const float a = us(16, 16, 1.2f, 0.10f), b = us(32, 32, 2.0f, 0.20f), c = us(32, 64, 3.0f, 0.29f);
+        if (us(128, 128, 6.0f, 0.31f) <= std::min(a, std::min(b, c))) return tile<128, 128, 2, 2>(x, w, out, st);
+        if (a <= std::min(b, c)) return direct<1, 1, 1, 8>(x, w, out, st);
+        if (b <= c) return direct<2, 2, 1, 8>(x, w, out, st);
     }
-    if (S >= 4) return direct<4, 4, 1, 4>(x, w, out, st);
+    if (S >= 4) return direct<2, 4, 1, 4>(x, w, out, st);
     return direct<4, 4, 4, 1>(x, w, out, st);
 }
 

@@ -172,7 +172,8 @@ def _small_rows(n, d, seed):
 @pytest.mark.parametrize("M,N,K", [(1, 1000, 128), (1, 70, 4096), (4, 333, 1024), (16, 500, 100), (31, 129, 768),
                                    (200, 300, 640), (513, 770, 96), (700, 260, 2000), (1030, 1100, 256),
                                    (3700, 3601, 640), (3850, 4001, 1060), (109, 33000, 130), (2100, 8200, 70),
-                           (1900, 2050, 4000)])
+                           (1900, 2050, 4000), (3, 50000, 100), (2, 49500, 700), (16, 13000, 1100), (5, 12500, 520),
+                           (7, 4500, 1100), (5, 33000, 1100), (130, 1900, 2100), (300, 3001, 600), (26, 1931, 1000)])
 def test_products_bit_for_bit(M, N, K):
     """Every product is a multiple of 1/16 and every partial sum below 2^20, so
     fp32 sums are exact in any order; a wrong element cannot hide."""
