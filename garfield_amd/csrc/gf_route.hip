@@ -170,40 +170,41 @@ __device__ __forceinline__ void wave_best(double& v, uint32_t& i) {
 }
 // A lane holds entries lane, lane + 64, ..: N of them.  Few rows come here, but a
 // launch waits for the last: its loads are in flight together and its keys in
-// registers (322 rows of 832 in bfloat16, whose groups tie now and then, with the
+// registers for the choices (322 rows of 832 in bfloat16, whose groups tie now and then, with the
 // gradient: 26 us; with keys read from LDS for every choice 102).
 // key: E doubles of LDS of this wave, for the groups' ranks.
 template <int N, class T>
 __device__ __attribute__((noinline)) void choose_exact(const gf_route_opts& o, const T* row, uint32_t E, const float* bias,
                                                        double* key, int32_t* chosen) {
     const uint32_t lane = threadIdx.x & 63u;
-    float l[N];
-    double mx = kNone, z = 0.0, x[N];
-    auto bias_of = [&](int n) { return bias && lane + 64u * n < E ? bias[lane + 64u * n] : 0.0f; };
-#pragma unroll
-    for (int n = 0; n < N; ++n) l[n] = lane + 64u * n < E ? float(row[lane + 64u * n]) : kNone;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {   // fmaxf takes a NaN for -inf
-        l[n] = bias_of(n) > kNone ? fminf(fmaxf(l[n], kNone), kLargest) : kNone;
-        mx = fmax(mx, double(l[n]));
+    double mx = kNone, z = 0.0;
+#pragma unroll 4
+    for (uint32_t e = lane; e < E; e += 64u) {   // a lane reads only what it wrote
+        const float l = entry(float(row[e]), bias, e);
+        key[e] = l;
+        mx = fmax(mx, double(l));
     }
     mx = wave_max(mx);
     const bool sigmoid = o.score == GF_SCORE_SIGMOID;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        x[n] = exp(sigmoid ? -double(l[n]) : double(l[n]) - (mx > kNone ? mx : 0.0));
-        z += l[n] > kNone ? x[n] : 0.0;
+    const double lift = mx > kNone ? mx : 0.0;
+#pragma unroll 1
+    for (uint32_t e = lane; e < E; e += 64u) {   // 0 for a masked entry of a softmax
+        const double v = key[e], x = exp(sigmoid ? -v : v - lift);
+        key[e] = v > kNone ? x : -1.0;
+        z += x;
     }
     z = wave_sum(z);
+#pragma unroll 1
+    for (uint32_t e = lane; e < E; e += 64u) {
+        const double x = key[e];
+        key[e] = x < 0.0 ? double(kNone) : (sigmoid ? 1.0 / (1.0 + x) : x / z) + (bias ? double(bias[e]) : 0.0);
+    }
+    double x[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-        x[n] = l[n] > kNone ? (sigmoid ? 1.0 / (1.0 + x[n]) : x[n] / z) + double(bias_of(n)) : double(kNone);
+    for (int n = 0; n < N; ++n) x[n] = lane + 64u * n < E ? key[lane + 64u * n] : double(kNone);
     if (o.groups > 1u) {
         const uint32_t gs = E / o.groups, share = 1u << (31 - __clz(int(64u / o.groups)));   // lanes a group
         const uint32_t g = lane / share, p = lane % share;
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-            if (lane + 64u * n < E) key[lane + 64u * n] = x[n];
         wave_lds_sync();
         double best = kNone, second = kNone;
         if (g < o.groups) {
@@ -248,13 +249,12 @@ __device__ __attribute__((noinline)) void choose_exact(const gf_route_opts& o, c
 
 // Dynamic LDS of k_route in words: the block's load counters; per wave the
 // chosen ids and the rows' keys and group ranks, or one row's keys in 64 bits.
-template <int LANES, int V, uint32_t WAVES>
+template <int LANES, int V>
 struct RouteLds {
     static constexpr uint32_t kRows = 64u / LANES;   // of a wave
     static constexpr uint32_t kKeys = LANES * V, kRow = kKeys + std::max<uint32_t>(GF_ROUTE_MAX_GROUPS, LANES * kGap<V>);
     static constexpr uint32_t kIds = kRows * GF_ROUTE_MAX_K;
     static constexpr uint32_t kWave = kIds + std::max(kRows * kRow, 2u * kKeys);
-    static constexpr uint32_t kBytes = 4u * (kKeys + WAVES * kWave);
 };
 
 // The three best of a lane's keys, the lower index first among equals (keys
@@ -274,26 +274,161 @@ struct Three {
     }
 };
 
-// A lane holds V consecutive entries of its row: the lowest lane that has the
-// largest key has the lowest index too.  It keeps its three best at hand and
-// looks through its V again only when all are chosen and it had more: with
-// k = 8 of 256 that is once in four rows.  Groups that are whole lanes are ranked
-// from the lanes' two best, by moves between lanes; others through LDS.
+// ---- sorted lists -------------------------------------------------------------
+// An entry is a double whose upper word is its key's bits and whose lower one is
+// its index, inverted under a positive key: doubles are ordered as floats are, by
+// sign and magnitude, so the larger double is the larger key or, among equal
+// keys, the lower index.  No key's bits reach a double's NaN (a float's infinity
+// is a finite double), and no two entries are equal.
+__device__ __forceinline__ double pack(float key, uint32_t index) {
+    const uint32_t hi = __float_as_uint(key + 0.0f);   // -0 is 0
+    const uint32_t lo = ~(index ^ uint32_t(int32_t(hi) >> 31));
+    return __longlong_as_double((long long)(uint64_t(hi) << 32 | lo));
+}
+__device__ __forceinline__ float key_of(double e) {
+    return __uint_as_float(uint32_t(uint64_t(__double_as_longlong(e)) >> 32));
+}
+__device__ __forceinline__ uint32_t index_of(double e) {
+    const uint64_t u = uint64_t(__double_as_longlong(e));
+    return ~(uint32_t(u) ^ uint32_t(int32_t(u >> 32) >> 31));
+}
+// Without the quieting of NaNs that fmax stands for.
+__device__ __forceinline__ double larger(double a, double b) {
+    double r;
+    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ double smaller(double a, double b) {
+    double r;
+    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ void in_order(double& a, double& b) {
+    const double x = larger(a, b);
+    b = smaller(a, b), a = x;
+}
+// Odd-even merge sort, largest first.
+template <int N>
+__device__ __forceinline__ void sort(double* a) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) in_order(a[i + j], a[i + j + k]);
+}
+// A list that falls and rises, largest first.
+template <int N>
+__device__ __forceinline__ void sort_bitonic(double* a) {
+#pragma unroll
+    for (int j = N / 2; j > 0; j /= 2)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!(i & j)) in_order(a[i], a[i | j]);
+}
+// The larger of two sorted lists' entries, at most LIST, sorted; `rest` the largest
+// of those that go.
+template <int LIST, int N>
+__device__ __forceinline__ void join(const double* a, const double* b, double* to, bool want_rest, double& rest) {
+    if constexpr (2 * N <= LIST) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) to[i] = a[i], to[2 * N - 1 - i] = b[i];
+        sort_bitonic<2 * N>(to);
+    } else {
+        if (want_rest) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) rest = larger(rest, smaller(a[i], b[N - 1 - i]));
+        }
+        double top[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) top[i] = larger(a[i], b[N - 1 - i]);
+        sort_bitonic<N>(top);
+#pragma unroll
+        for (int i = 0; i < N; ++i) to[i] = top[i];
+    }
+}
+template <int LIST, int N>
+constexpr int kJoined = 2 * N <= LIST ? 2 * N : LIST;
+// Each lane's N entries, joined over the row's lanes: LIST of them in every lane.
+template <int LIST, int CTRL, int N>
+__device__ __forceinline__ void join_turned(double* a, bool want_rest, double& rest) {
+    double b[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) b[i] = dpp64<CTRL>(a[i]);
+    if (want_rest) rest = larger(rest, dpp64<CTRL>(rest));
+    double own[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) own[i] = a[i];
+    join<LIST, N>(own, b, a, want_rest, rest);
+}
+template <bool HALVES>   // lanes ^ 32, or lanes ^ 16
+__device__ __forceinline__ void both_sides(double v, double& a, double& b) {
+    const uint64_t u = uint64_t(__double_as_longlong(v));
+    const uint32_t lo = uint32_t(u), hi = uint32_t(u >> 32);
+    uint32_t l[2], h[2];
+    if constexpr (HALVES) {
+        const auto x = __builtin_amdgcn_permlane32_swap(lo, lo, false, false), y = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+        l[0] = x[0], l[1] = x[1], h[0] = y[0], h[1] = y[1];
+    } else {
+        const auto x = __builtin_amdgcn_permlane16_swap(lo, lo, false, false), y = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+        l[0] = x[0], l[1] = x[1], h[0] = y[0], h[1] = y[1];
+    }
+    a = __longlong_as_double((long long)(uint64_t(h[0]) << 32 | l[0]));
+    b = __longlong_as_double((long long)(uint64_t(h[1]) << 32 | l[1]));
+}
+template <int LIST, bool HALVES>
+__device__ __forceinline__ void join_swapped(double* a, bool want_rest, double& rest) {
+    double x[LIST], y[LIST];
+#pragma unroll
+    for (int i = 0; i < LIST; ++i) both_sides<HALVES>(a[i], x[i], y[i]);
+    if (want_rest) {
+        double p, q;
+        both_sides<HALVES>(rest, p, q);
+        rest = larger(p, q);
+    }
+    join<LIST, LIST>(x, y, a, want_rest, rest);
+}
+template <int LIST, int LANES, int N>
+__device__ __forceinline__ void join_row(double* a, bool want_rest, double& rest) {
+    constexpr int A = kJoined<LIST, N>, B = kJoined<LIST, A>, C = kJoined<LIST, B>;
+    join_turned<LIST, 0x128, N>(a, want_rest, rest);
+    join_turned<LIST, 0x124, A>(a, want_rest, rest);
+    join_turned<LIST, 0x122, B>(a, want_rest, rest);
+    join_turned<LIST, 0x121, C>(a, want_rest, rest);
+    static_assert(kJoined<LIST, C> == LIST, "");
+    if constexpr (LANES == 64) {
+        join_swapped<LIST, false>(a, want_rest, rest);
+        join_swapped<LIST, true>(a, want_rest, rest);
+    }
+}
+
+// A lane holds V consecutive entries of its row.  For 4 to 16 choices it sorts
+// its own into a list of LIST and the row's lanes join theirs, in four (six) steps
+// whose cost does not depend on k: every lane ends with the row's list.  Else
+// (LIST = 0) the row's best is taken k times: a lane keeps its three best at hand,
+// the lowest lane that has the largest key has the lowest index too, and it looks
+// through its V again only when all three are chosen and it had more.  Groups
+// that are whole lanes are ranked from the lanes' two best, by moves between
+// lanes; others through LDS.
 //
-// What bounds it is the instructions issued, some 460 a row of 256, not the 1 KB
-// read: 10,000 rows of 256 in 32 bits, k = 8 by logit, take 14 us (8 us with k = 1),
-// 17 us with 4 of 16 groups kept, 22 us with the load and the launch that clears it;
-// 16,384 rows by sigmoid and bias in 8 groups 31 us.  A whole wave for a row
-// of more than 256 (8 or 16 entries a lane instead of 32 or 64, a quarter of the
+// What bounds it is the instructions issued, not the bytes read: 10,000 rows of
+// 256 in 32 bits, k = 8 by logit, 4 of 16 groups kept, take 15 us with the load and
+// the launch that clears it (21 by the loop), 16,384 rows by sigmoid and bias in 8
+// groups 25 us (31); what they read takes 2 and 4.  A whole wave for a row of more
+// than 256 (8 or 16 entries a lane instead of 32 or 64, a quarter of the
 // registers) took 28 us for 4 rows of 1008 where sixteen lanes took 71, 62 for
-// 10,636 rows of 1018 where they took 73, 90 for 25,564 of 455 where they took 93.
-template <class T, int LANES, int V, uint32_t WAVES>
-__global__ __launch_bounds__(64 * WAVES, 4) void k_route(gf_route_opts o, const T* logits, uint32_t rows, uint32_t E,
+// 10,636 rows of 1018 where they took 73.
+template <class T, int LANES, int V, int LIST>
+__global__ __launch_bounds__(1024) void k_route(gf_route_opts o, const T* logits, uint32_t rows, uint32_t E,
                                                          uint64_t ld, const float* bias, int32_t* ids, float* weights,
                                                          int32_t* load) {
     extern __shared__ __align__(16) uint32_t lds[];
-    using L = RouteLds<LANES, V, WAVES>;
+    using L = RouteLds<LANES, V>;
     constexpr uint32_t kRows = L::kRows;
+    const uint32_t waves = blockDim.x >> 6;
     const uint32_t lane = threadIdx.x & 63u, c = lane % LANES, mine = lane / LANES, wave = threadIdx.x >> 6;
     const uint32_t first = c * V;
     uint32_t* count = lds;
@@ -302,7 +437,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_route(gf_route_opts o, const 
     float* keys = reinterpret_cast<float*>(own + L::kIds);
     float *mykeys = keys + mine * L::kRow, *myranks = mykeys + L::kKeys;
     if (load) {
-        for (uint32_t e = threadIdx.x; e < E; e += 64u * WAVES) count[e] = 0;
+        for (uint32_t e = threadIdx.x; e < E; e += blockDim.x) count[e] = 0;
         __syncthreads();
     }
     const bool by_score = bias || (o.groups > 1u && o.group_score == GF_GROUP_TOP2);
@@ -312,8 +447,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_route(gf_route_opts o, const 
     const uint32_t span = whole ? 16u / o.groups : 1u;
     const uint32_t gs = E / o.groups, magic = ((1u << 20) + gs - 1u) / gs;   // e / gs = e magic >> 20 below 1024
 
-    for (uint64_t t0 = (uint64_t(blockIdx.x) * WAVES + wave) * kRows; t0 < rows;
-         t0 += uint64_t(gridDim.x) * WAVES * kRows) {
+    for (uint64_t t0 = (uint64_t(blockIdx.x) * waves + wave) * kRows; t0 < rows;
+         t0 += uint64_t(gridDim.x) * waves * kRows) {
         const bool row_ok = t0 + mine < rows;
         const uint64_t t = row_ok ? t0 + mine : rows - 1u;   // lanes without a row repeat the last, unstored
         const T* row = logits + t * ld;
@@ -380,8 +515,32 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_route(gf_route_opts o, const 
             }
         }
         bool close = false;   // a comparison that 32 bits do not decide
+        constexpr int kOwn = V < LIST ? V : LIST > 0 ? LIST : 1;   // entries of the lane's own list
+        double list[LIST > 0 ? LIST : 1], rest = pack(kNone, 0);
         Three best;
-        best.clear();
+        // the lane's best entries of key[]
+        auto gather = [&] {
+            if constexpr (LIST > 0) {
+                double all[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) all[j] = pack(key[j], first + j);
+#pragma unroll
+                for (int j = 0; j < V; j += kOwn) sort<kOwn>(all + j);
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) list[j] = all[j];
+#pragma unroll
+                for (int j = kOwn; j < V; j += kOwn) {
+                    double own[kOwn];
+#pragma unroll
+                    for (int i = 0; i < kOwn; ++i) own[i] = list[i];
+                    join<LIST, kOwn>(own, all + j, list, by_score, rest);
+                }
+            } else {
+                best.clear();
+#pragma unroll
+                for (int j = 0; j < V; ++j) best.add(key[j], first + j);
+            }
+        };
         auto rank_of = [&](float first_best, float second_best) {
             return first_best + (o.group_score == GF_GROUP_TOP2 && second_best > kNone ? second_best : 0.0f);
         };
@@ -391,10 +550,13 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_route(gf_route_opts o, const 
             return by_score && high > kNone && low - high <= 2.0f * (off(fabsf(low) + top) + off(fabsf(high) + top));
         };
         if (o.groups == 1u || whole) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) best.add(key[j], first + j);
+            gather();
             if (whole) {
-                float u = best.v[0], d = best.v[1];
+                float u, d;
+                if constexpr (LIST > 0)
+                    u = key_of(list[0]), d = V > 1 ? key_of(list[V > 1 ? 1 : 0]) : kNone;
+                else
+                    u = best.v[0], d = best.v[1];
                 for (uint32_t s = 1; s < span; s <<= 1) {
                     const float u2 = __shfl_xor(u, int(s)), d2 = __shfl_xor(d, int(s));
                     d = fmaxf(fmaxf(d, d2), fminf(u, u2));
@@ -412,7 +574,13 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_route(gf_route_opts o, const 
                 }
                 const bool kept = ahead < o.keep_groups * span;
                 close = too_close(-max_row<LANES>(kept ? -rank : kNone), max_row<LANES>(kept ? kNone : rank));
-                if (!kept) best.clear();
+                if constexpr (LIST > 0) {
+#pragma unroll
+                    for (int j = 0; j < kOwn; ++j) list[j] = kept ? list[j] : pack(kNone, 0);
+                    rest = kept ? rest : pack(kNone, 0);
+                } else if (!kept) {
+                    best.clear();
+                }
             }
         } else {
 #pragma unroll
@@ -472,48 +640,63 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_route(gf_route_opts o, const 
                 const bool over = --left == 0;
                 g += over, left = over ? gs : left;
             }
-#pragma unroll
-            for (int j = 0; j < V; ++j) best.add(key[j], first + j);
+            gather();
         }
-        float before = 0.0f;
-        bool more = best.v[2] > kNone;   // the lane may have a fourth
-        for (uint32_t n = 0; n <= o.k; ++n) {
-            const float m = max_row<LANES>(best.v[0]);
-            const uint64_t who = ballot_row<LANES>(best.v[0] == m && m > kNone);
-            if (by_score && n) {
-                bool near = who && before - m <= off(before) + off(m);
-                if (__any(near)) {   // the same logit and bias: an exact tie, the lower index first
-                    wave_lds_sync();
-                    const uint32_t at = __shfl(best.i[0], int(mine * LANES + (who ? uint32_t(__ffsll((long long)who)) - 1u : 0u)));
-                    const uint32_t last = near ? uint32_t(chosen[n - 1u]) : 0u;
-                    if (near && row[at] == row[last] && (!bias || bias[at] == bias[last])) near = false;
-                }
-                close |= near;
-            }
-            before = m;
-            if (n == o.k) break;
-            if (!who && c == 0) chosen[n] = -1;
-            if (who && c == uint32_t(__ffsll((long long)who)) - 1u) {
-                const uint32_t last = best.i[0];
-                chosen[n] = int32_t(last);
-                best.v[0] = best.v[1], best.i[0] = best.i[1];
-                best.v[1] = best.v[2], best.i[1] = best.i[2];
-                best.v[2] = kNone;
-                if (V > 3 && more && !(best.v[0] > kNone)) {   // look again, behind (m, last)
-                    best.clear();
+        // the same logit and bias: an exact tie, the lower index first
+        auto tied = [&](uint32_t a, uint32_t b) { return row[a] == row[b] && (!bias || bias[a] == bias[b]); };
+        if constexpr (LIST > 0) {
+            join_row<LIST, LANES, kOwn>(list, by_score, rest);
+            // lane n has the list's entry n, and the one behind it
+            double here = list[0], next = list[1];
 #pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        best.add(key[j] < m || (key[j] == m && first + j > last) ? key[j] : kNone, first + j);
-                    more = best.v[2] > kNone;
+            for (int n = 1; n < LIST; ++n) {
+                here = c == uint32_t(n) ? list[n] : here;
+                next = c == uint32_t(n) ? n + 1 < LIST ? list[n + 1 < LIST ? n + 1 : 0] : rest : next;
+            }
+            const float v = key_of(here), w = key_of(next);
+            if (by_score && c < o.k && w > kNone && v - w <= off(v) + off(w))
+                close |= !tied(index_of(here), index_of(next));
+            if (c < o.k) chosen[c] = v > kNone ? int32_t(index_of(here)) : -1;
+        } else {
+            float before = 0.0f;
+            bool more = best.v[2] > kNone;   // the lane may have a fourth
+            for (uint32_t n = 0; n <= o.k; ++n) {
+                const float m = max_row<LANES>(best.v[0]);
+                const uint64_t who = ballot_row<LANES>(best.v[0] == m && m > kNone);
+                if (by_score && n) {
+                    bool near = who && before - m <= off(before) + off(m);
+                    if (__any(near)) {
+                        wave_lds_sync();
+                        const uint32_t at = __shfl(best.i[0], int(mine * LANES + (who ? uint32_t(__ffsll((long long)who)) - 1u : 0u)));
+                        if (near && tied(at, uint32_t(chosen[n - 1u]))) near = false;
+                    }
+                    close |= near;
+                }
+                before = m;
+                if (n == o.k) break;
+                if (!who && c == 0) chosen[n] = -1;
+                if (who && c == uint32_t(__ffsll((long long)who)) - 1u) {
+                    const uint32_t last = best.i[0];
+                    chosen[n] = int32_t(last);
+                    best.v[0] = best.v[1], best.i[0] = best.i[1];
+                    best.v[1] = best.v[2], best.i[1] = best.i[2];
+                    best.v[2] = kNone;
+                    if (V > 3 && more && !(best.v[0] > kNone)) {   // look again, behind (m, last)
+                        best.clear();
+#pragma unroll
+                        for (int j = 0; j < V; ++j)
+                            best.add(key[j] < m || (key[j] == m && first + j > last) ? key[j] : kNone, first + j);
+                        more = best.v[2] > kNone;
+                    }
                 }
             }
         }
         wave_lds_sync();
         if (by_score) {
-            uint64_t again = __ballot(close && c == 0);
+            uint64_t again = __ballot(close);
             while (again) {
                 const uint32_t r = uint32_t(__ffsll((long long)again) - 1) / LANES;
-                again &= again - 1u;
+                again &= LANES == 64 ? 0u : ~(0xFFFFull << (r * 16u));   // the row's lanes
                 choose_exact<(LANES * V + 63) / 64>(o, logits + min(t0 + r, uint64_t(rows) - 1u) * ld, E, bias, reinterpret_cast<double*>(keys),
                              reinterpret_cast<int32_t*>(own) + r * GF_ROUTE_MAX_K);
             }
@@ -547,7 +730,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_route(gf_route_opts o, const 
     }
     if (load) {   // whole numbers: the order does not matter
         __syncthreads();
-        for (uint32_t e = threadIdx.x; e < E; e += 64u * WAVES)
+        for (uint32_t e = threadIdx.x; e < E; e += blockDim.x)
             if (count[e]) atomicAdd(load + e, int32_t(count[e]));
     }
 }
@@ -698,21 +881,24 @@ hipError_t launch_route(const gf_route_opts& opts, const MatIn& logits, uint32_t
         return by_width(E, [&](auto lanes, auto width) {
             using T = decltype(v);
             constexpr int kLanes = decltype(lanes)::value, V = decltype(width)::value;
-            using L4 = RouteLds<kLanes, V, 4>;
-            auto go = [&](auto waves) {
-                constexpr uint32_t W = decltype(waves)::value;
-                using L = RouteLds<kLanes, V, W>;
-                hipLaunchKernelGGL((k_route<T, kLanes, V, W>), dim3(route_blocks(logits.rows, W, L::kRows)), 64 * W,
-                                   L::kBytes, st, o, static_cast<const T*>(logits.p), uint32_t(logits.rows), E, logits.ld,
-                                   bias, ids, weights, load);
+            using L = RouteLds<kLanes, V>;
+            auto go = [&](auto lists, uint32_t waves) {
+                hipLaunchKernelGGL((k_route<T, kLanes, V, decltype(lists)::value>),
+                                   dim3(route_blocks(logits.rows, waves, L::kRows)), 64u * waves,
+                                   4u * (L::kKeys + waves * L::kWave), st, o, static_cast<const T*>(logits.p),
+                                   uint32_t(logits.rows), E, logits.ld, bias, ids, weights, load);
                 return hipGetLastError();
             };
             // A block ends with an atomic addition for every entry that it counted: where
             // rows fill the chip anyway, few large blocks (4096 rows of 512 with the load
-            // 17 us against 22, 10,000 of 256 18.5 against 19.9 by blocks of eight waves).
-            if (load && (logits.rows + L4::kRows - 1u) / L4::kRows >= 2048u)
-                return go(std::integral_constant<uint32_t, 16>());
-            return go(std::integral_constant<uint32_t, 4>());
+            // 16 us against 20, 10,000 of 512 25 against 37).
+            const uint32_t waves = load && (logits.rows + L::kRows - 1u) / L::kRows >= 2048u ? 16u : 4u;
+            // Lists cost the same for every k, a turn of the loop for every entry.  32,768
+            // rows of 256 and of 896, by lists against the loop: k = 2 27.0 us against 27.8 and
+            // 59 against 59, k = 8 27 against 37 and 64 against 88, k = 16 33 against 59 and
+            // 86 against 119.
+            if (o.k < 4u || o.k > 16u) return go(std::integral_constant<int, 0>(), waves);
+            return o.k <= 8u ? go(std::integral_constant<int, 8>(), waves) : go(std::integral_constant<int, 16>(), waves);
         });
     });
 }

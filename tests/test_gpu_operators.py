@@ -388,7 +388,9 @@ def test_route_ties_and_near_ties(score):
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("E,groups,keep,k", [(12, 4, 2, 5), (120, 8, 8, 30), (256, 16, 4, 8), (300, 1, 1, 64), (320, 10, 4, 9),
-                                             (512, 64, 20, 16), (1000, 8, 3, 12), (1024, 1, 1, 1)])
+                                             (512, 64, 20, 16), (1000, 8, 3, 12), (1024, 1, 1, 1), (16, 1, 1, 16),
+                                             (16, 16, 9, 8), (60, 1, 1, 4), (64, 8, 3, 8), (250, 2, 1, 13), (400, 1, 1, 8),
+                                             (700, 7, 7, 3), (1024, 16, 16, 16), (777, 1, 1, 17)])
 def test_route_ties_of_rounded_logits(E, groups, keep, k, score):
     """Logits of few values: equal sums of score and bias, equal ranks of groups,
     in rows of every width; bias none, nothing, or of few values."""
