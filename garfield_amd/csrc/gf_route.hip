@@ -174,7 +174,7 @@ __device__ __forceinline__ void wave_best(double& v, uint32_t& i) {
 // gradient: 26 us; with keys read from LDS for every choice 102).
 // key: E doubles of LDS of this wave, for the groups' ranks.
 template <int N, class T>
-__device__ __attribute__((noinline)) void choose_exact(const gf_route_opts& o, const T* row, uint32_t E, const float* bias,
+__device__ __attribute__((noinline)) void choose_exact(gf_route_opts o, const T* row, uint32_t E, const float* bias,
                                                        double* key, int32_t* chosen) {
     const uint32_t lane = threadIdx.x & 63u;
     double mx = kNone, z = 0.0;
