@@ -16,8 +16,8 @@ template <int DT>
 constexpr int kPlanes = DT == GF_BF16 ? 1 : DT == GF_F16 ? 2 : 3;
 
 // The planes of eight values: the leading 8 bits, the next 8, the last.  An
-// infinity or NaN lies in the first alone; no remainder exceeds the value, so
-// none overflows.
+// infinity or NaN lies in the first alone (a NaN quieted, so that the upper half
+// keeps a bit of its payload); no remainder exceeds the value, so none overflows.
 template <int P>
 __device__ __forceinline__ void split8(const float* v, uint4* plane) {
     uint32_t out[P][4];
@@ -26,19 +26,17 @@ __device__ __forceinline__ void split8(const float* v, uint4* plane) {
         uint32_t top[P][2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            float rest = v[i + k];
-            const uint32_t bits = __float_as_uint(rest);
-            const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
-            // a NaN keeps a bit of its payload in the upper half
-            top[0][k] = (bits & 0x7FFFFFFFu) > 0x7F800000u ? bits | 0x00400000u : bits;
+            const float whole = __builtin_canonicalizef(v[i + k]);
+            float rest = __builtin_isfinite(whole) ? whole : 0.0f;
+            top[0][k] = __float_as_uint(whole);
 #pragma unroll
             for (int p = 1; p < P; ++p) {
-                rest -= __uint_as_float((p == 1 ? bits : top[p - 1][k]) & 0xFFFF0000u);
-                top[p][k] = finite ? __float_as_uint(rest) : 0u;
+                rest -= __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
+                top[p][k] = __float_as_uint(rest);
             }
         }
 #pragma unroll
-        for (int p = 0; p < P; ++p) out[p][i / 2] = top[p][0] >> 16 | (top[p][1] & 0xFFFF0000u);
+        for (int p = 0; p < P; ++p) out[p][i / 2] = __builtin_amdgcn_perm(top[p][1], top[p][0], 0x07060302u);   // upper halves
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) plane[p] = make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
@@ -198,10 +196,10 @@ __global__ __launch_bounds__(64 * WK) void k_mx_few(const ElemT<DT>* x, uint32_t
 // comes through registers, one block of 32 values a thread, decoded on its way
 // to LDS, loaded one step ahead (two slots).  A real side in bfloat16 (or in
 // planes, one after the other) comes by copies straight to LDS, two steps ahead
-// (three slots; COPIED); one in binary16 or fp32, or whose rows are not whole
-// steps, through registers, split into its planes on its way, one step ahead (two
-// slots): a small result is then one launch, and the planes share what is read
-// and decoded of the other side.  A
+// (three slots; COPIED).  In tiles of 64 it comes through registers in its own
+// type, split into its planes on its way, one step ahead (two slots): a small
+// result is then one launch, whose rows need not be aligned or whole steps, and
+// the planes share what is read and decoded of the other side.  A
 // step has four parts; a part's operands are read from LDS while the part before
 // it is multiplied, across steps too.
 // Columns are rows of w (TR = false: the product) or positions in w's rows
@@ -298,13 +296,17 @@ __global__ __launch_bounds__(64 * VM * VN) void k_mx_real(RealArgs p, ElemT<OT>*
         if constexpr (!COPIED) {
 #pragma unroll
             for (uint32_t i = 0; i < kPer; ++i) {
-                ElemT<DT> e[8];
-                __builtin_memcpy(e, raw[i], sizeof(e));
-                float v[8];
-#pragma unroll
-                for (int c = 0; c < 8; ++c) v[c] = float(e[c]);
                 uint4 plane[P];
-                split8<P>(v, plane);
+                if constexpr (DT == GF_BF16) {
+                    plane[0] = raw[i][0];
+                } else {
+                    ElemT<DT> e[8];
+                    __builtin_memcpy(e, raw[i], sizeof(e));
+                    float v[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) v[c] = float(e[c]);
+                    split8<P>(v, plane);
+                }
 #pragma unroll
                 for (int q = 0; q < P; ++q)
                     *reinterpret_cast<uint4*>(lds + slot * L::kA + q * L::kPlane + (i * TH + tid) * 16u) = plane[q];
@@ -509,19 +511,19 @@ uint32_t planes_of(int32_t dtype) { return dtype == GF_BF16 ? 1u : dtype == GF_F
 // the smaller ones) and once what a tile takes besides; a launch and 7 TB/s for
 // planes and for joining parts, which are read back from the caches for the most
 // part.  Fitted to 168 products and gradients of 17 to 10,000 real rows with each
-// tile: nine in ten of its times are within 15% of the measured one, and the
-// tile it takes was 1% slower than the best on average and 18% at most.  Large,
-// small, split: fp32, 4096 x 8192 x 4096 721, 867, 935 us, 2048 x 2048 x 4096 120,
-// 148, 135; binary16, 1024 x 53124 x 1024 212, 223, 328, the gradient of 777
-// queries over 9376 rows of 100 38, 27, 20, in bfloat16 31, 23, 18; bfloat16, 4096 x
-// 8192 x 4096 217, 282, 2048 x 2048 x 4096 57, 45.
+// tile: six in seven of its times are within 15% of the measured one, and the
+// tile it takes was 1% slower than the best on average and 17% at most.  Large,
+// small, split: fp32, 4096 x 8192 x 4096 721, 867, 830 us, 2048 x 2048 x 4096 121, 153,
+// 122; binary16, 1024 x 53124 x 1024 212, 222, 289, the gradient of 777 queries over
+// 9376 rows of 100 38, 26, 19, in bfloat16 31, 23, 17; bfloat16, 4096 x 8192 x 4096
+// 217, 275, 380, 64 x 53124 x 1024 31, 22, 17.
 struct TileCost {
     float one, two, besides;
 };
 constexpr TileCost kTileCost[3][3] = {   // by tile, by type (GF_F32, GF_F16, GF_BF16)
     {{1.75f, 1.75f, 6.0f}, {1.51f, 1.51f, 6.0f}, {1.62f, 1.62f, 6.0f}},
     {{0.72f, 1.06f, 2.2f}, {0.65f, 1.00f, 2.2f}, {0.67f, 1.06f, 2.2f}},
-    {{1.16f, 2.02f, 2.2f}, {0.99f, 1.60f, 2.0f}, {0.80f, 1.25f, 1.2f}}};
+    {{1.00f, 1.74f, 2.2f}, {0.85f, 1.30f, 2.0f}, {0.52f, 0.79f, 1.2f}}};
 constexpr float kLaunch = 3.0f, kByte = 1.0f / 7e6f;
 RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
     RealPlan best = {};
@@ -529,7 +531,6 @@ RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
     const uint64_t steps = (J + 63u) / 64u;
     const bool in_steps = dtype == GF_BF16 && J % 64u == 0;   // read in place where aligned
     for (const Tile tile : {kLarge, kSmall, kSplit}) {
-        if (tile == kSplit && in_steps) continue;
         const uint64_t bm = tile == kLarge ? 256u : tile == kSmall ? 128u : 64u, bn = tile == kLarge ? 256u : 128u;
         const uint64_t tm = (M + bm - 1u) / bm, tn = (N + bn - 1u) / bn, planes = tile == kSplit ? 1u : planes_of(dtype);
         uint64_t parts = std::min<uint64_t>((tile == kSplit ? 2u : 1u) * kUnits / (tm * tn), steps / 4u);
