@@ -495,8 +495,8 @@ uint32_t blocks_for(uint64_t items) { return uint32_t(std::min<uint64_t>((items 
 
 // How a product of M real rows of J values with N columns runs: the tile, the
 // real side as planes or split in the kernel, and the sum in parts where the
-// tiles leave compute units idle (at least four steps of 64 a part, and no more
-// partial sums than 64 MiB).  The plan is part of the interface (the workspace's
+// tiles leave compute units idle (up to six blocks a unit, at least four steps of
+// 64 a part, and no more partial sums than 64 MiB).  The plan is part of the interface (the workspace's
 // size), so it is made for the chip's compute units, not the current device's.
 constexpr uint64_t kUnits = 256;
 enum Tile { kLarge, kSmall, kSplit };
@@ -506,13 +506,15 @@ struct RealPlan {
     uint32_t tm, tn, parts;
 };
 uint32_t planes_of(int32_t dtype) { return dtype == GF_BF16 ? 1u : dtype == GF_F16 ? 2u : 3u; }
-// The plan is the tile whose time, in us, is the least by this account: rounds of
+// The plan is the one whose time, in us, is the least by this account: rounds of
 // the chip's tiles, for each a step's time (one tile on a compute unit; two of
 // the smaller ones) and once what a tile takes besides; a launch and 7 TB/s for
 // planes and for joining parts, which are read back from the caches for the most
-// part.  Fitted to 168 products and gradients of 17 to 10,000 real rows with each
-// tile: six in seven of its times are within 15% of the measured one, and the
-// tile it takes was 1% slower than the best on average and 17% at most.  Large,
+// part.  Fitted to 240 products and gradients of 17 to 10,000 real rows with each
+// tile: five in six of its times are within 15% of the measured one, and the
+// tile it takes was 1% slower than the best on average and 18% at most.  Parts up
+// to one block a unit instead: the gradient of 4077 rows in fp32 over 5678 rows of
+// 365 93 us against 75, 2759 over 31907 of 514 508 against 421.  Large,
 // small, split: fp32, 4096 x 8192 x 4096 721, 867, 830 us, 2048 x 2048 x 4096 121, 153,
 // 122; binary16, 1024 x 53124 x 1024 212, 222, 289, the gradient of 777 queries over
 // 9376 rows of 100 38, 26, 19, in bfloat16 31, 23, 17; bfloat16, 4096 x 8192 x 4096
@@ -533,19 +535,24 @@ RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
     for (const Tile tile : {kLarge, kSmall, kSplit}) {
         const uint64_t bm = tile == kLarge ? 256u : tile == kSmall ? 128u : 64u, bn = tile == kLarge ? 256u : 128u;
         const uint64_t tm = (M + bm - 1u) / bm, tn = (N + bn - 1u) / bn, planes = tile == kSplit ? 1u : planes_of(dtype);
-        uint64_t parts = std::min<uint64_t>((tile == kSplit ? 2u : 1u) * kUnits / (tm * tn), steps / 4u);
-        parts = std::max<uint64_t>(std::min<uint64_t>(parts, (16u << 20) / (M * N)), 1u);
         const TileCost& c = kTileCost[tile][dtype];
-        const uint64_t tiles = tm * tn * parts, round = tile == kLarge ? kUnits : 2u * kUnits;
-        const uint64_t full = tiles / round, rest = tiles % round;
-        const float step = float(full) * c.two + (rest == 0 ? 0.0f : rest <= kUnits ? c.one : c.two);
-        float us = step * float((steps * planes + parts - 1u) / parts) + c.besides * float(full + (rest != 0));
-        if (tile != kSplit && !in_steps)
-            us += kLaunch + float(M) * float(J) * float(dtype == GF_F32 ? 10 : dtype == GF_F16 ? 6 : 4) * kByte;
-        if (parts > 1u) us += kLaunch + float(M) * float(N) * float(parts) * 8.0f * kByte;
-        if (best.tm && us >= least) continue;
-        least = us;
-        best = {tile, tile != kSplit, uint32_t(tm), uint32_t(tn), uint32_t(parts)};
+        const uint64_t round = tile == kLarge ? kUnits : 2u * kUnits;
+        uint64_t last = 0;
+        for (uint64_t units = kUnits; units <= 6u * kUnits; units += kUnits) {
+            uint64_t parts = std::min<uint64_t>(units / (tm * tn), steps / 4u);
+            parts = std::max<uint64_t>(std::min<uint64_t>(parts, (16u << 20) / (M * N)), 1u);
+            if (parts == last) continue;
+            last = parts;
+            const uint64_t tiles = tm * tn * parts, full = tiles / round, rest = tiles % round;
+            const float step = float(full) * c.two + (rest == 0 ? 0.0f : rest <= kUnits ? c.one : c.two);
+            float us = step * float((steps * planes + parts - 1u) / parts) + c.besides * float(full + (rest != 0));
+            if (tile != kSplit && !in_steps)
+                us += kLaunch + float(M) * float(J) * float(dtype == GF_F32 ? 10 : dtype == GF_F16 ? 6 : 4) * kByte;
+            if (parts > 1u) us += kLaunch + float(M) * float(N) * float(parts) * 8.0f * kByte;
+            if (best.tm && us >= least) continue;
+            least = us;
+            best = {tile, tile != kSplit, uint32_t(tm), uint32_t(tn), uint32_t(parts)};
+        }
     }
     return best;
 }
