@@ -417,7 +417,7 @@ __device__ __forceinline__ void join_row(double* a, bool want_rest, double& rest
 // What bounds it is the instructions issued, not the bytes read: 10,000 rows of
 // 256 in 32 bits, k = 8 by logit, 4 of 16 groups kept, take 15 us with the load and
 // the launch that clears it (21 by the loop), 16,384 rows by sigmoid and bias in 8
-// groups 25 us (31); what they read takes 2 and 4.  A whole wave for a row of more
+// groups 23 us (30); what they read takes 2 and 4.  A whole wave for a row of more
 // than 256 (8 or 16 entries a lane instead of 32 or 64, a quarter of the
 // registers) took 28 us for 4 rows of 1008 where sixteen lanes took 71, 62 for
 // 10,636 rows of 1018 where they took 73.
@@ -742,7 +742,10 @@ __global__ void k_route_clear(int32_t* load, uint32_t E) {
 
 // The gradient, sixteen lanes a row as above: the k chosen entries' terms are
 // put into a row of LDS that is written out whole; the softmax over all
-// entries adds its term to every live one.
+// entries adds its term to every live one.  16,384 rows of 256 in 32 bits, 8
+// chosen: 7 us, 2.4 TB/s of gradient, bound by the chain from ids over logits to
+// the sums; 15,287 rows of 992 with the softmax over all 74 us (177 with each
+// exponential taken twice), bound by the exponentials.
 constexpr uint32_t kGradWaves = 4, kGradRows = 4;   // a block's waves, a wave's rows
 template <class T>
 __global__ __launch_bounds__(64 * kGradWaves) void k_route_grad(gf_route_opts o, const T* logits, uint32_t rows, uint32_t E,
@@ -876,7 +879,8 @@ hipError_t launch_route(const gf_route_opts& opts, const MatIn& logits, uint32_t
     }
     if (!logits.rows) return hipSuccess;
     gf_route_opts o = opts;
-    if (o.keep_groups == o.groups) o.groups = o.keep_groups = 1;   // all groups: the same as none
+    // all groups: the same as none, but for GF_GROUP_TOP2's order by score
+    if (o.keep_groups == o.groups && (bias || o.group_score == GF_GROUP_MAX)) o.groups = o.keep_groups = 1;
     return by_type(logits.dtype, [&](auto v) {
         return by_width(E, [&](auto lanes, auto width) {
             using T = decltype(v);

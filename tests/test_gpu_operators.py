@@ -409,6 +409,22 @@ def test_route_ties_of_rounded_logits(E, groups, keep, k, score):
             _close(got.weights, w, orc.WEIGHT_RTOL * np.abs(w) + 2.0 ** -126, "weights")
 
 
+@pytest.mark.parametrize("keep", [2, 4])
+def test_route_saturated_sigmoids(keep):
+    """Sigmoids that are 1 in 64 bits tie where entries are ranked by score, not
+    where they are by logit."""
+    _case("saturated", keep)
+    l = torch.arange(64, dtype=torch.float32).repeat(5, 1) + 40.0
+    l[1:, ::3] = -60.0
+    for rank in ("max", "top2"):
+        for bias in (None, torch.zeros(64)):
+            got = gf.route(l.cuda(), 6, bias=None if bias is None else bias.cuda(), score="sigmoid", groups=4,
+                           keep_groups=keep, group_score=rank)
+            ids, _, _ = orc.route(l.numpy(), 6, bias=None if bias is None else bias.numpy(), score="sigmoid", groups=4,
+                                  keep_groups=keep, group_score=rank)
+            assert np.array_equal(_np(got.ids), ids)
+
+
 def test_route_grad_ignores_foreign_ids():
     _case("foreign ids")
     l = _rows(4, 16, torch.float32, 1, spread=False)
