@@ -14,6 +14,7 @@ row distance; their last dimension must be contiguous.  Every call raises if
 the library is missing; there is no other code path.
 """
 import ctypes as C
+import functools
 
 from . import _lib
 
@@ -93,16 +94,36 @@ class MXRows:
                 raise ValueError(f"{what} must be a contiguous (rows, {width}) uint8 tensor on the GPU")
             if t.data_ptr() % align:
                 raise ValueError(f"{what} must be aligned to {align} bytes")
-        self._set(codes, scales, int(K))
+        self._parts = codes, scales
+        self.K, self.rows, self.device = int(K), codes.shape[0], codes.device
+        self._struct = _lib.MXRowsStruct(codes.data_ptr(), scales.data_ptr(), self.rows, self.K)
 
-    def _set(self, codes, scales, K):
-        self.codes, self.scales, self.K, self.rows = codes, scales, K, codes.shape[0]
-        self._struct = _lib.MXRowsStruct(codes.data_ptr(), scales.data_ptr(), self.rows, K)
+    @classmethod
+    def _allocate(cls, rows, K, device):
+        """Rows to be written: codes and scales one after the other in one
+        allocation, split when somebody asks for them."""
+        self = cls.__new__(cls)
+        S = -(-K // 128)
+        self._parts = torch.empty(rows * (68 * S), dtype=torch.uint8, device=device)
+        self.K, self.rows, self.device = K, rows, device
+        at = self._parts.data_ptr()
+        self._struct = _lib.MXRowsStruct(at, at + rows * (64 * S), rows, K)
         return self
 
+    def _split(self):
+        if not isinstance(self._parts, tuple):
+            S = -(-self.K // 128)
+            codes, scales = self._parts.split((self.rows * 64 * S, self.rows * 4 * S))
+            self._parts = codes.view(self.rows, 64 * S), scales.view(self.rows, 4 * S)
+        return self._parts
+
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self):
+        return self._split()[0]
+
+    @property
+    def scales(self):
+        return self._split()[1]
 
     def __getitem__(self, rows):
         """A run of whole rows (a slice of step 1), such as one cell's, without a copy."""
@@ -116,12 +137,9 @@ def mx_quantise(x):
     t, n, K, ld = _matrix(x, "x")
     if K < 1:
         raise ValueError("x must have at least one column")
-    S = -(-K // 128)
-    dev = x.device
-    codes = torch.empty((n, 64 * S), dtype=torch.uint8, device=dev)
-    scales = torch.empty((n, 4 * S), dtype=torch.uint8, device=dev)
-    _call(dev, _lib.load().gf_mx_quantise, x.data_ptr(), t, n, K, ld, codes.data_ptr(), scales.data_ptr())
-    return MXRows.__new__(MXRows)._set(codes, scales, K)
+    w = MXRows._allocate(n, K, x.device)
+    _call(w.device, _lib.load().gf_mx_quantise, x.data_ptr(), t, n, K, ld, w._struct.codes, w._struct.scales)
+    return w
 
 
 def mx_dequantise(w, dtype=None):
@@ -136,12 +154,16 @@ def mx_dequantise(w, dtype=None):
     return out
 
 
-def _workspace(kind, t, M, w):
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(kind, t, M, rows, K):
     n = C.c_size_t()
-    _lib._check(_lib.load().gf_mx_product_workspace(kind, t, M, w.rows, w.K, C.byref(n)))
-    if not n.value:
-        return None, 0
-    return torch.empty(n.value, dtype=torch.uint8, device=w.device), n.value
+    _lib._check(_lib.load().gf_mx_product_workspace(kind, t, M, rows, K, C.byref(n)))
+    return n.value
+
+
+def _workspace(kind, t, M, w):
+    n = _workspace_bytes(kind, t, M, w.rows, w.K)
+    return (torch.empty(n, dtype=torch.uint8, device=w.device), n) if n else (None, 0)
 
 
 def _product(x, w, dtype):
