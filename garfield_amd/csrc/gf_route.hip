@@ -731,7 +731,10 @@ __global__ __launch_bounds__(1024) void k_route(gf_route_opts o, const T* logits
     if (load) {   // whole numbers: the order does not matter
         __syncthreads();
         for (uint32_t e = threadIdx.x; e < E; e += blockDim.x)
-            if (count[e]) atomicAdd(load + e, int32_t(count[e]));
+            if (gridDim.x == 1u)
+                load[e] = int32_t(count[e]);
+            else if (count[e])
+                atomicAdd(load + e, int32_t(count[e]));
     }
 }
 
@@ -873,11 +876,11 @@ uint32_t route_blocks(uint64_t rows, uint32_t waves, uint32_t rows_of_wave) {
 
 hipError_t launch_route(const gf_route_opts& opts, const MatIn& logits, uint32_t E, const float* bias, int32_t* ids,
                         float* weights, int32_t* load, hipStream_t st) {
-    if (load) {
-        hipLaunchKernelGGL(k_route_clear, dim3((E + 255u) / 256u), 256, 0, st, load, E);
-        if (const hipError_t e = hipGetLastError()) return e;
-    }
-    if (!logits.rows) return hipSuccess;
+    auto clear = [&] {
+        if (load) hipLaunchKernelGGL(k_route_clear, dim3((E + 255u) / 256u), 256, 0, st, load, E);
+        return hipGetLastError();
+    };
+    if (!logits.rows) return clear();
     gf_route_opts o = opts;
     // all groups: the same as none, but for GF_GROUP_TOP2's order by score
     if (o.keep_groups == o.groups && (bias || o.group_score == GF_GROUP_MAX)) o.groups = o.keep_groups = 1;
@@ -886,23 +889,30 @@ hipError_t launch_route(const gf_route_opts& opts, const MatIn& logits, uint32_t
             using T = decltype(v);
             constexpr int kLanes = decltype(lanes)::value, V = decltype(width)::value;
             using L = RouteLds<kLanes, V>;
-            auto go = [&](auto lists, uint32_t waves) {
+            const uint64_t all = (logits.rows + L::kRows - 1u) / L::kRows;   // waves with rows
+            // A block ends with an atomic addition for every entry that it counted: where
+            // rows fill the chip anyway, few large blocks (4096 rows of 512 with the load
+            // 16 us against 20, 10,000 of 512 25 against 37).  One block alone writes its
+            // counts, and nothing need be cleared before it: 16 rows of 256, back to back 11.6
+            // us against 14.2, a call alone 22.1 against 24.4 (64 rows, 16 waves: 26.1
+            // against 24.6).
+            const bool alone = load && all <= 8u;
+            const uint32_t waves = alone ? uint32_t(all) : load && all >= 2048u ? 16u : 4u;
+            if (!alone)
+                if (const hipError_t e = clear()) return e;
+            auto go = [&](auto lists) {
                 hipLaunchKernelGGL((k_route<T, kLanes, V, decltype(lists)::value>),
-                                   dim3(route_blocks(logits.rows, waves, L::kRows)), 64u * waves,
+                                   dim3(alone ? 1u : route_blocks(logits.rows, waves, L::kRows)), 64u * waves,
                                    4u * (L::kKeys + waves * L::kWave), st, o, static_cast<const T*>(logits.p),
                                    uint32_t(logits.rows), E, logits.ld, bias, ids, weights, load);
                 return hipGetLastError();
             };
-            // A block ends with an atomic addition for every entry that it counted: where
-            // rows fill the chip anyway, few large blocks (4096 rows of 512 with the load
-            // 16 us against 20, 10,000 of 512 25 against 37).
-            const uint32_t waves = load && (logits.rows + L::kRows - 1u) / L::kRows >= 2048u ? 16u : 4u;
             // Lists cost the same for every k, a turn of the loop for every entry.  32,768
             // rows of 256 and of 896, by lists against the loop: k = 2 27.0 us against 27.8 and
             // 59 against 59, k = 8 27 against 37 and 64 against 88, k = 16 33 against 59 and
             // 86 against 119.
-            if (o.k < 4u || o.k > 16u) return go(std::integral_constant<int, 0>(), waves);
-            return o.k <= 8u ? go(std::integral_constant<int, 8>(), waves) : go(std::integral_constant<int, 16>(), waves);
+            if (o.k < 4u || o.k > 16u) return go(std::integral_constant<int, 0>());
+            return o.k <= 8u ? go(std::integral_constant<int, 8>()) : go(std::integral_constant<int, 16>());
         });
     });
 }

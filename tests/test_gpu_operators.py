@@ -310,7 +310,7 @@ ROUTES = [
     dict(T=25, E=12, k=3, groups=4, keep_groups=1), dict(T=25, E=64, k=5, groups=64, keep_groups=9, group_score="top2"),
     dict(T=19, E=96, k=12, groups=3, keep_groups=2, group_score="top2", bias=True),
     dict(T=17, E=1024, k=16, groups=2, keep_groups=1, bias=True, group_score="top2"), dict(T=1, E=256, k=8, bias=True),
-    dict(T=1000, E=160, k=6, groups=5, keep_groups=2),
+    dict(T=1000, E=160, k=6, groups=5, keep_groups=2), dict(T=32, E=200, k=9), dict(T=8, E=300, k=3), dict(T=9, E=300, k=4),
 ]
 
 
