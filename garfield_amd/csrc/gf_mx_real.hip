@@ -637,9 +637,9 @@ hipError_t launch_mx_product(const MatIn& x, const gf_mx_rows& w, const MatOut& 
             // so a split goes with more rows.  One query, <1, 1>, <2, 1>, <2, 4>, <1, 8>:
             // bfloat16, 53124 rows of 1024 8.3, 8.1, 13.6, 15.2 us, 16384 of 4096 14.2, 17.6,
             // 9.5, 10.6, 2000 of 8000 26, 33, 12, 8; binary16, <1, 1>, <4, 1>, <4, 4>, <4, 8>,
-            // <2, 8>, <1, 8>: 300000 of 100 21, 12, 20, 41, 58, 101; 200000 of 2000 153, 99,
-            // 76, 93, 115, 188; 16384 of 4096 35, 48, 18, 16, 18, 26; 8192 of 4096 31, 46, 17,
-            // 15, 12, 15; 2000 of 8000 63, 94, 32, 25, 21, 18.
+            // <2, 8>, <1, 8>: 300000 of 100 16, 11, 19, 37, 50, 78; 200000 of 2000 94, 80, 67,
+            // 83, 98, 125; 16384 of 4096 24, 42, 16, 13, 14, 16; 8192 of 4096 21, 38, 15, 12,
+            // 9, 10; 2000 of 8000 45, 74, 28, 20, 16, 13.
             const std::integral_constant<int, 1> one;
             const std::integral_constant<int, 2> two;
             const std::integral_constant<int, 4> four;
