@@ -533,6 +533,7 @@ constexpr TileCost kTileCost[3][3] = {   // by tile, by type (GF_F32, GF_F16, GF
     {{0.72f, 1.06f, 2.2f}, {0.65f, 1.00f, 2.2f}, {0.67f, 1.06f, 2.2f}},
     {{1.00f, 1.74f, 2.2f}, {0.85f, 1.30f, 2.0f}, {0.52f, 0.79f, 1.2f}}};
 constexpr float kLaunch = 3.0f, kByte = 1.0f / 7e6f;
+constexpr float kMostPlanes = 4294967296.0f;   // bytes; beyond, the kernel splits and needs none
 RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
     RealPlan best = {};
     float least = 0.0f;
@@ -541,6 +542,7 @@ RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
     for (const Tile tile : {kLarge, kSmall, kSplit}) {
         const uint64_t bm = tile == kLarge ? 256u : tile == kSmall ? 128u : 64u, bn = tile == kLarge ? 256u : 128u;
         const uint64_t tm = (M + bm - 1u) / bm, tn = (N + bn - 1u) / bn, planes = tile == kSplit ? 1u : planes_of(dtype);
+        if (tile != kSplit && !in_steps && float(M) * float(steps) * float(planes) * 128.0f > kMostPlanes) continue;
         const TileCost& c = kTileCost[tile][dtype];
         const uint64_t round = tile == kLarge ? kUnits : 2u * kUnits;
         uint64_t last = 0;

@@ -94,6 +94,16 @@ def test_workspace_is_checked():
     assert lib.gf_mx_product_workspace(0, 0, 1, 1, 1, None) == ARG
 
 
+def test_workspace_of_large_calls_is_bounded():
+    """Beyond 4 GiB of planes the real side is split where it is used."""
+    n = C.c_size_t()
+    for dtype in (0, 1):
+        assert _lib.load().gf_mx_product_workspace(0, dtype, 1 << 22, 8192, 4096, C.byref(n)) == 0
+        assert n.value == 0
+        assert _lib.load().gf_mx_product_workspace(0, dtype, 1 << 16, 8192, 4096, C.byref(n)) == 0
+        assert 0 < n.value <= 4 << 30
+
+
 def _opts(**kw):
     o = dict(k=4, score=0, groups=1, keep_groups=1, group_score=0, renormalise=1, scale=1.0)
     o.update(kw)
