@@ -118,7 +118,18 @@ __device__ __forceinline__ float entry(float l, const float* bias, uint32_t e) {
 
 // exp to 2^-17 of itself or better, below 2^-126 0.
 __device__ __forceinline__ float exp_near(float v) { return __builtin_amdgcn_exp2f(v * 1.4426950408889634f); }
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
+// e^-lift times the sigmoid of v, lift being 0 or, if v is below -17, at least v.
+// There the sigmoid is e^v, but for less than 2^-24 of itself; 1 / (1 + e^-v) would
+// be 0 from -88.8 on.  Below 2^-1022 it counts as 0: entries at a type's lowest value.
+constexpr float kLeastSigmoid = -708.39642f;
+__device__ __forceinline__ float sigmoid(float v, float lift = 0.0f) {
+    const bool low = v < -17.0f;
+    const float e = expf(low ? v - lift : -v);
+    return low ? v < kLeastSigmoid ? 0.0f : e : 1.0f / (1.0f + e);
+}
+// The lift of a row whose largest chosen logit is top, where weights are shares of
+// the chosen sigmoids' sum: shares of what need not underflow.
+__device__ __forceinline__ float sigmoid_lift(float top) { return top < -17.0f ? top : 0.0f; }
 
 // ---- one row by the whole wave, keys in 64 bits --------------------------------
 template <int CTRL>
@@ -712,9 +723,10 @@ __global__ __launch_bounds__(1024) void k_route(gf_route_opts o, const T* logits
             peak = fmaxf(peak, l[i]);
         }
         if (o.renormalise) mx = max_row<LANES>(peak);   // the softmax over the row cancels
+        const float from = o.renormalise ? sigmoid_lift(mx) : 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < kChoices; ++i) {
-            s[i] = id[i] < 0 ? 0.0f : soft ? expf(l[i] - mx) / (o.renormalise ? 1.0f : z) : sigmoid(l[i]);
+            s[i] = id[i] < 0 ? 0.0f : soft ? expf(l[i] - mx) / (o.renormalise ? 1.0f : z) : sigmoid(l[i], from);
             sum += s[i];
         }
         if (o.renormalise) sum = sum_row<LANES>(sum);
@@ -794,9 +806,10 @@ __global__ __launch_bounds__(64 * kGradWaves) void k_route_grad(gf_route_opts o,
         } else {
             mx = max16(peak), z = 1.0f;
         }
+        const float from = o.renormalise ? sigmoid_lift(mx) : 0.0f;   // (sigmoids)
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
-            s[i] = id[i] < 0 ? 0.0f : soft ? expf(l[i] - mx) / z : sigmoid(l[i]);
+            s[i] = id[i] < 0 ? 0.0f : soft ? expf(l[i] - mx) / z : sigmoid(l[i], from);
             sum += s[i];
         }
         float mean = 0.0f;
@@ -808,7 +821,8 @@ __global__ __launch_bounds__(64 * kGradWaves) void k_route_grad(gf_route_opts o,
             for (uint32_t i = 0; i < 4u; ++i) share[i] = s[i] * inv, mean += g[i] * share[i];
             mean = sum16(mean);
 #pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) g[i] = o.scale * (g[i] - mean) * share[i] * (soft ? 1.0f : 1.0f - s[i]);
+            for (uint32_t i = 0; i < 4u; ++i)   // below -17 a sigmoid's 1 - s is 1
+                g[i] = o.scale * (g[i] - mean) * share[i] * (soft || l[i] < -17.0f ? 1.0f : 1.0f - s[i]);
         } else if (soft) {
 #pragma unroll
             for (uint32_t i = 0; i < 4u; ++i) mean += g[i] * s[i];

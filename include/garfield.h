@@ -514,7 +514,8 @@ gf_status gf_mx_product_workspace(int32_t kind, int32_t dtype, uint64_t M, uint6
 /* Routing of T queries (tokens) to k of E cells (experts) each.  An entry is
  * live when its logit, and its bias if there is one, is neither -inf nor NaN
  * (a logit of +inf counts as the largest finite one).  Scores are the softmax
- * over a row's live logits, or their sigmoids.  Entries are ranked by score +
+ * over a row's live logits, or their sigmoids (one below 2^-1022, of a logit
+ * below -708.4, counts as 0 in the weights).  Entries are ranked by score +
  * bias, compared as in exact arithmetic (64 bits), ties to the lower index;
  * with neither a bias nor GF_GROUP_TOP2 by the logit itself.  With groups > 1
  * (E / groups consecutive entries each) only the keep_groups best groups are
