@@ -20,6 +20,7 @@ from . import _lib
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORES = {"max": 0, "top2": 1}
+MAX_CHOICES = 64    # of a row of route (GF_ROUTE_MAX_K)
 torch = None        # imported by the first call: the rest of the package does without
 _types = {}
 

@@ -7,8 +7,10 @@ keeps the k best of those that the query's range allows, and the search visits
 these alone (``Batch.set_cells``).
 
 - training: ``mx_product`` of the mapped queries with the centres, ``route``'s
-  softmax weights, and their gradients (``mx_product_grad``, ``route_grad``
-  behind autograd) through the frozen centres to the map;
+  softmax weights (of more than 64 cells, which ``route`` does not choose at
+  once, the cross entropy of the scores), and their gradients
+  (``mx_product_grad``, ``route_grad`` behind autograd) through the frozen
+  centres to the map;
 - serving: the mapped queries quantised (``mx_quantise``), both sides at four
   bits, cells outside a range masked, at most ``keep_groups`` of ``groups`` runs
   of cells (shards) a query.
@@ -24,7 +26,7 @@ from . import operators as ops
 
 
 class CellRouter:
-    """Scores of P cells for D-dimensional queries: (q @ map) . centre / temperature."""
+    """Scores of P cells, at most 1024, for D-dimensional queries: (q @ map) . centre / temperature."""
 
     def __init__(self, centres, temperature=0.1, seed=0):
         """centres: (P, D) mean vectors of the cells, on the GPU; kept at four bits."""
@@ -45,9 +47,12 @@ class CellRouter:
         losses = []
         for _ in range(steps):
             logits = ops.mx_product(queries @ self.map, self.centres) / self.temperature
-            r = ops.route(logits, self.centres.rows)       # all cells, best first
-            weight = torch.where(r.ids == target[:, None], r.weights, 0).sum(1)
-            loss = -weight.clamp_min(1e-20).log().mean()
+            if self.centres.rows <= ops.MAX_CHOICES:
+                r = ops.route(logits, self.centres.rows)   # all cells, best first
+                weight = torch.where(r.ids == target[:, None], r.weights, 0).sum(1)
+                loss = -weight.clamp_min(1e-20).log().mean()
+            else:                                          # a target need not be among the best
+                loss = torch.nn.functional.cross_entropy(logits, target)
             opt.zero_grad(set_to_none=True)
             loss.backward()
             opt.step()
