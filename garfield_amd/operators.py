@@ -21,6 +21,7 @@ from . import _lib
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORES = {"max": 0, "top2": 1}
 MAX_CHOICES = 64    # of a row of route (GF_ROUTE_MAX_K)
+_MAX_SIZE = 0x7FFFFF00     # rows or columns: the library counts them in 32 bits
 torch = None        # imported by the first call: the rest of the package does without
 _types = {}
 
@@ -46,9 +47,11 @@ def _matrix(x, what):
     """x as the library reads it: (type, rows, columns, row distance)."""
     if not isinstance(x, _need_torch().Tensor) or x.ndim != 2:
         raise ValueError(f"{what} must be a matrix (a 2-d tensor)")
+    n, d = x.shape
+    if d > _MAX_SIZE:
+        raise ValueError(f"{what} must have at most {_MAX_SIZE} columns")
     if not x.is_cuda:
         raise ValueError(f"{what} must be on the GPU")
-    n, d = x.shape
     ld, one = x.stride()
     if one != 1 and d > 1:
         raise ValueError(f"{what}'s last dimension must be contiguous")
@@ -59,10 +62,22 @@ def _matrix(x, what):
     return _type(x.dtype, what), n, d, ld
 
 
+def _count(x, what):
+    """A whole number that the library's 32 bits hold."""
+    try:
+        n = int(x)
+    except (TypeError, ValueError, OverflowError):
+        n = -1
+    if n != x or not 0 <= n <= _MAX_SIZE:
+        raise ValueError(f"{what} must be a whole number from 0 to {_MAX_SIZE}, got {x!r}")
+    return n
+
+
 def _vector(x, shape, dtype, device, what):
     if x is None:
         return None
-    if x.shape != shape or x.dtype != dtype or x.device != device or not x.is_contiguous():
+    if (not isinstance(x, torch.Tensor) or x.shape != shape or x.dtype != dtype or x.device != device
+            or not x.is_contiguous()):
         raise ValueError(f"{what} must be a contiguous {tuple(shape)} {dtype} tensor on {device}")
     return x.data_ptr()
 
@@ -85,7 +100,8 @@ class MXRows:
 
     def __init__(self, codes, scales, K):
         _need_torch()
-        S = -(-int(K) // 128)
+        K = _count(K, "K")
+        S = -(-K // 128)
         if K < 1:
             raise ValueError("K must be at least 1")
         for t, width, align, what in ((codes, 64 * S, 16, "codes"), (scales, 4 * S, 4, "scales")):
@@ -96,7 +112,7 @@ class MXRows:
             if t.data_ptr() % align:
                 raise ValueError(f"{what} must be aligned to {align} bytes")
         self._parts = codes, scales
-        self.K, self.rows, self.device = int(K), codes.shape[0], codes.device
+        self.K, self.rows, self.device = K, codes.shape[0], codes.device
         self._struct = _lib.MXRowsStruct(codes.data_ptr(), scales.data_ptr(), self.rows, self.K)
 
     @classmethod
@@ -283,12 +299,14 @@ def _choice(table, key, what):
 
 def _route(logits, k, bias, groups, keep_groups, group_score, score, renormalise, scale):
     t, T, E, ld = _matrix(logits, "logits")
-    opts = _lib.RouteOpts(int(k), _choice(_SCORES, score, "score"), int(groups), int(keep_groups),
+    k = _count(k, "k")
+    opts = _lib.RouteOpts(k, _choice(_SCORES, score, "score"), _count(groups, "groups"), _count(keep_groups, "keep_groups"),
                           _choice(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalise)), float(scale))
     b = _vector(bias, (E,), torch.float32, logits.device, "bias")
     dev = logits.device
-    ids = torch.empty((T, max(int(k), 0)), dtype=torch.int32, device=dev)
-    weights = torch.empty((T, max(int(k), 0)), dtype=torch.float32, device=dev)
+    # of a k that is refused, nothing is allocated
+    ids = torch.empty((T, k if k <= MAX_CHOICES else 0), dtype=torch.int32, device=dev)
+    weights = torch.empty((T, k if k <= MAX_CHOICES else 0), dtype=torch.float32, device=dev)
     load = torch.empty((E,), dtype=torch.int32, device=dev)
     _call(dev, _lib.load().gf_route, C.byref(opts), logits.data_ptr(), t, T, E, ld, b, ids.data_ptr(),
           weights.data_ptr(), load.data_ptr())
@@ -313,9 +331,9 @@ def route_grad(logits, ids, dweights, bias=None, score="softmax", renormalise=Tr
     the logits' type, from dweights (T, k) float32 and route's ids; bias, score,
     renormalise and scale as in the call of route (gf_route_grad)."""
     t, T, E, ld = _matrix(logits, "logits")
-    if ids.ndim != 2:
-        raise ValueError("ids must be (T, k)")
-    k = ids.shape[1]
+    if not isinstance(ids, torch.Tensor) or ids.ndim != 2:
+        raise ValueError("ids must be a (T, k) tensor")
+    k = _count(ids.shape[1], "k")
     dev = logits.device
     i = _vector(ids, (T, k), torch.int32, dev, "ids")
     g = _vector(dweights, (T, k), torch.float32, dev, "dweights")
