@@ -127,6 +127,12 @@ class MXRows:
         self._struct = _lib.MXRowsStruct(at, at + rows * (64 * S), rows, K)
         return self
 
+    def _versions(self):
+        """What grows when the codes or scales are written to, but for tensors
+        of inference mode, which keep no count."""
+        codes, scales = self._split()
+        return tuple(0 if t.is_inference() else t._version for t in (codes, scales))
+
     def _split(self):
         if not isinstance(self._parts, tuple):
             S = -(-self.K // 128)
@@ -236,12 +242,18 @@ def _autograd():
         class Product(torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, w, dtype):
+                out = _product(x, w, dtype)
                 ctx.w, ctx.dtype = w, x.dtype
-                return _product(x, w, dtype)
+                ctx.rows_as_they_were = w._versions()
+                return out
 
             @staticmethod
             @torch.autograd.function.once_differentiable
             def backward(ctx, dy):
+                # not by save_for_backward, which takes no tensors of inference mode
+                if ctx.rows_as_they_were != ctx.w._versions():
+                    raise RuntimeError("mx_product: the rows have been modified by an inplace operation since the "
+                                       "forward pass")
                 if dy.ndim == 2 and dy.shape[1] > 1 and dy.stride(1) != 1 or dy.stride(0) < dy.shape[1]:
                     dy = dy.contiguous()
                 return mx_product_grad(dy, ctx.w, ctx.dtype), None, None
