@@ -151,6 +151,8 @@ _SYMBOLS = {
     "gf_mx_product_grad": [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint64, C.POINTER(MXRowsStruct), C.c_int32,
                            C.c_void_p, C.c_uint64, C.c_void_p, C.c_size_t, C.c_void_p],
     "gf_mx_product_workspace": [C.c_int32, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint32, C.POINTER(C.c_size_t)],
+    "gf_mx_product_workspace_at": [C.c_int32, C.c_void_p, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32,
+                                   C.POINTER(C.c_size_t)],
     "gf_route": [C.POINTER(RouteOpts), C.c_void_p, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint64, C.c_void_p,
                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
     "gf_route_grad": [C.POINTER(RouteOpts), C.c_void_p, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint64, C.c_void_p,

@@ -508,7 +508,7 @@ constexpr uint64_t kUnits = 256;
 enum Tile { kLarge, kSmall, kSplit };
 struct RealPlan {
     Tile tile;
-    bool planes;   // the real side as planes in the workspace
+    bool planes;   // the real side as planes in the workspace, not read in place or split
     uint32_t tm, tn, parts;
 };
 uint32_t planes_of(int32_t dtype) { return dtype == GF_BF16 ? 1u : dtype == GF_F16 ? 2u : 3u; }
@@ -533,16 +533,16 @@ constexpr TileCost kTileCost[3][3] = {   // by tile, by type (GF_F32, GF_F16, GF
     {{0.72f, 1.06f, 2.2f}, {0.65f, 1.00f, 2.2f}, {0.67f, 1.06f, 2.2f}},
     {{1.00f, 1.74f, 2.2f}, {0.85f, 1.30f, 2.0f}, {0.52f, 0.79f, 1.2f}}};
 constexpr float kLaunch = 3.0f, kByte = 1.0f / 7e6f;
-constexpr float kMostPlanes = 4294967296.0f;   // bytes; beyond, the kernel splits and needs none
-RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
+constexpr uint64_t kMostPlanes = 1ull << 32;   // bytes; beyond, the kernel splits and needs none
+// in_place: the real side is read where it lies.
+RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J, bool in_place) {
     RealPlan best = {};
     float least = 0.0f;
     const uint64_t steps = (J + 63u) / 64u;
-    const bool in_steps = dtype == GF_BF16 && J % 64u == 0;   // read in place where aligned
     for (const Tile tile : {kLarge, kSmall, kSplit}) {
         const uint64_t bm = tile == kLarge ? 256u : tile == kSmall ? 128u : 64u, bn = tile == kLarge ? 256u : 128u;
         const uint64_t tm = (M + bm - 1u) / bm, tn = (N + bn - 1u) / bn, planes = tile == kSplit ? 1u : planes_of(dtype);
-        if (tile != kSplit && !in_steps && float(M) * float(steps) * float(planes) * 128.0f > kMostPlanes) continue;
+        if (tile != kSplit && !in_place && M > kMostPlanes / (steps * planes * 128u)) continue;
         const TileCost& c = kTileCost[tile][dtype];
         const uint64_t round = tile == kLarge ? kUnits : 2u * kUnits;
         uint64_t last = 0;
@@ -554,30 +554,34 @@ RealPlan real_plan(int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
             const uint64_t tiles = tm * tn * parts, full = tiles / round, rest = tiles % round;
             const float step = float(full) * c.two + (rest == 0 ? 0.0f : rest <= kUnits ? c.one : c.two);
             float us = step * float((steps * planes + parts - 1u) / parts) + c.besides * float(full + (rest != 0));
-            if (tile != kSplit && !in_steps)
+            if (tile != kSplit && !in_place)
                 us += kLaunch + float(M) * float(J) * float(dtype == GF_F32 ? 10 : dtype == GF_F16 ? 6 : 4) * kByte;
             if (parts > 1u) us += kLaunch + float(M) * float(N) * float(parts) * 8.0f * kByte;
             if (best.tm && us >= least) continue;
             least = us;
-            best = {tile, tile != kSplit, uint32_t(tm), uint32_t(tn), uint32_t(parts)};
+            best = {tile, tile != kSplit && !in_place, uint32_t(tm), uint32_t(tn), uint32_t(parts)};
         }
     }
     return best;
 }
-// Whether a bfloat16 side can be read in place: rows of whole steps, aligned
-// for the copies.
-bool in_place(const MatIn& a, uint64_t J) {
-    return a.dtype == GF_BF16 && J % 64u == 0 && a.ld % 8u == 0 && reinterpret_cast<uintptr_t>(a.p) % 16u == 0 && a.ld < 1u << 22;
+// Whether a side of J values a row can be read in place: bfloat16, rows of whole
+// steps, aligned for the copies.
+bool in_place(int32_t dtype, const void* p, uint64_t ld, uint64_t J) {
+    return dtype == GF_BF16 && J % 64u == 0 && ld % 8u == 0 && reinterpret_cast<uintptr_t>(p) % 16u == 0 && ld < 1u << 22;
+}
+size_t plan_bytes(const RealPlan& pl, int32_t dtype, uint64_t M, uint64_t N, uint64_t J) {
+    return (pl.planes ? size_t((J + 63u) / 64u) * 128u * planes_of(dtype) * M : 0u) +
+           (pl.parts > 1u ? size_t(pl.parts) * M * N * 4u : 0u);
 }
 
 template <bool TR>
 hipError_t real_product(const MatIn& a, uint64_t J, const gf_mx_rows& w, uint64_t N, const MatOut& out, void* ws,
                         hipStream_t st) {
-    const RealPlan pl = real_plan(a.dtype, a.rows, N, J);
+    const RealPlan pl = real_plan(a.dtype, a.rows, N, J, in_place(a.dtype, a.p, a.ld, J));
     if (!grid_fits(uint64_t(pl.tm) * pl.tn * pl.parts, 512u)) return hipErrorInvalidConfiguration;
     RealArgs p = {a.p, a.ld, 64, uint32_t(a.rows), uint32_t(J), 1u, w, mx_chunks(w.K), uint32_t(N), pl.tm, pl.tn, pl.parts};
     uint8_t* at = static_cast<uint8_t*>(ws);
-    if (pl.planes && !in_place(a, J)) {
+    if (pl.planes) {
         const uint32_t steps = uint32_t((J + 63u) / 64u);
         p.a = at, p.lda = 64, p.step = a.rows * 64u, p.planes = planes_of(a.dtype);
         const hipError_t e = by_type(a.dtype, [&](auto dt) {
@@ -674,10 +678,14 @@ hipError_t launch_mx_product_grad(const MatIn& dy, const gf_mx_rows& w, const Ma
 size_t mx_workspace(int32_t kind, int32_t dtype, uint64_t M, uint64_t rows, uint32_t K) {
     if (kind == 1 || !M || !rows || (kind == 0 && M <= kFew)) return 0;
     const uint64_t J = kind == 2 ? rows : K, N = kind == 2 ? K : rows;
-    const RealPlan pl = real_plan(dtype, M, N, J);
-    // bfloat16: room for the rows by steps, whether or not they can be read in place
-    return (pl.planes ? size_t((J + 63u) / 64u) * 128u * planes_of(dtype) * M : 0u) +
-           (pl.parts > 1u ? size_t(pl.parts) * M * N * 4u : 0u);
+    size_t most = plan_bytes(real_plan(dtype, M, N, J, false), dtype, M, N, J);
+    if (in_place(dtype, nullptr, 0, J)) most = std::max(most, plan_bytes(real_plan(dtype, M, N, J, true), dtype, M, N, J));
+    return most;
+}
+size_t mx_workspace(int32_t kind, const MatIn& x, uint64_t rows, uint32_t K) {
+    if (kind == 1 || !x.rows || !rows || (kind == 0 && x.rows <= kFew)) return 0;
+    const uint64_t J = kind == 2 ? rows : K, N = kind == 2 ? K : rows;
+    return plan_bytes(real_plan(x.dtype, x.rows, N, J, in_place(x.dtype, x.p, x.ld, J)), x.dtype, x.rows, N, J);
 }
 
 }  // namespace gf

@@ -49,8 +49,8 @@ void check_rows(const gf_mx_rows* w, const char* what) {
                GF_E_ARG, std::string(what) + ": codes must be aligned to 16 bytes, scales to 4");
 }
 
-void check_workspace(int32_t kind, int32_t dtype, uint64_t M, const gf_mx_rows& w, const void* ws, size_t bytes) {
-    const size_t need = gf::mx_workspace(kind, dtype, M, w.rows, w.K);
+void check_workspace(int32_t kind, const gf::MatIn& x, const gf_mx_rows& w, const void* ws, size_t bytes) {
+    const size_t need = gf::mx_workspace(kind, x, w.rows, w.K);
     GF_REQUIRE(bytes >= need && (ws || !need), GF_E_ARG,
                "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
     GF_REQUIRE(!need || reinterpret_cast<uintptr_t>(ws) % 16 == 0, GF_E_ARG, "workspace must be aligned to 16 bytes");
@@ -110,7 +110,7 @@ gf_status gf_mx_product(const void* x, int32_t dtype, uint64_t M, uint64_t ldx, 
         check_rows(w, "w");
         check_matrix(x, dtype, M, w->K, ldx, "x");
         check_matrix(out, out_dtype, M, w->rows, ldo, "out");
-        check_workspace(0, dtype, M, *w, workspace, workspace_bytes);
+        check_workspace(0, {x, dtype, M, ldx}, *w, workspace, workspace_bytes);
         if (!M || !w->rows) return;
         launched(gf::launch_mx_product({x, dtype, M, ldx}, *w, {out, out_dtype, ldo}, workspace, hipStream_t(stream)));
     });
@@ -123,7 +123,7 @@ gf_status gf_mx_product_mx(const gf_mx_rows* x, const gf_mx_rows* w, int32_t out
         check_rows(w, "w");
         GF_REQUIRE(x->K == w->K, GF_E_ARG, "x and w hold different numbers of values a row");
         check_matrix(out, out_dtype, x->rows, w->rows, ldo, "out");
-        check_workspace(1, GF_F32, x->rows, *w, workspace, workspace_bytes);
+        check_workspace(1, {nullptr, GF_F32, x->rows, 0}, *w, workspace, workspace_bytes);
         if (!x->rows || !w->rows) return;
         launched(gf::launch_mx_product_mx(*x, *w, {out, out_dtype, ldo}, workspace, hipStream_t(stream)));
     });
@@ -136,7 +136,7 @@ gf_status gf_mx_product_grad(const void* dy, int32_t dtype, uint64_t M, uint64_t
         check_rows(w, "w");
         check_matrix(dy, dtype, M, w->rows, ldy, "dy");
         check_matrix(dx, out_dtype, M, w->K, ldo, "dx");
-        check_workspace(2, dtype, M, *w, workspace, workspace_bytes);
+        check_workspace(2, {dy, dtype, M, ldy}, *w, workspace, workspace_bytes);
         if (!M) return;
         launched(gf::launch_mx_product_grad({dy, dtype, M, ldy}, *w, {dx, out_dtype, ldo}, workspace,
                                           hipStream_t(stream)));
@@ -150,6 +150,17 @@ gf_status gf_mx_product_workspace(int32_t kind, int32_t dtype, uint64_t M, uint6
         GF_REQUIRE(dtype >= GF_F32 && dtype <= GF_BF16, GF_E_ARG, "unknown element type");
         GF_REQUIRE(M <= kMaxRows && rows <= kMaxRows && K >= 1 && K <= kMaxRows, GF_E_ARG, "sizes out of range");
         *bytes = gf::mx_workspace(kind, dtype, M, rows, K);
+    });
+}
+
+gf_status gf_mx_product_workspace_at(int32_t kind, const void* x, int32_t dtype, uint64_t M, uint64_t ldx, uint64_t rows,
+                                     uint32_t K, size_t* bytes) {
+    return guarded([&] {
+        GF_REQUIRE(bytes, GF_E_ARG, "null argument");
+        GF_REQUIRE(kind >= 0 && kind <= 2, GF_E_ARG, "unknown kind");
+        GF_REQUIRE(dtype >= GF_F32 && dtype <= GF_BF16, GF_E_ARG, "unknown element type");
+        GF_REQUIRE(M <= kMaxRows && rows <= kMaxRows && K >= 1 && K <= kMaxRows, GF_E_ARG, "sizes out of range");
+        *bytes = gf::mx_workspace(kind, {x, dtype, M, ldx}, rows, K);
     });
 }
 

@@ -33,8 +33,11 @@ hipError_t launch_mx_product(const MatIn& x, const gf_mx_rows& w, const MatOut& 
 hipError_t launch_mx_product_mx(const gf_mx_rows& x, const gf_mx_rows& w, const MatOut& out, void* ws,
                                 hipStream_t st);
 hipError_t launch_mx_product_grad(const MatIn& dy, const gf_mx_rows& w, const MatOut& dx, void* ws, hipStream_t st);
-// Workspace bytes by kind (0 product, 1 both at four bits, 2 gradient).
+// Workspace bytes by kind (0 product, 1 both at four bits, 2 gradient): enough
+// for M real rows wherever they lie, and those of one call (of x its address and
+// row distance count, its values are not read).
 size_t mx_workspace(int32_t kind, int32_t dtype, uint64_t M, uint64_t rows, uint32_t K);
+size_t mx_workspace(int32_t kind, const MatIn& x, uint64_t rows, uint32_t K);
 
 hipError_t launch_route(const gf_route_opts& o, const MatIn& logits, uint32_t E, const float* bias, int32_t* ids,
                         float* weights, int32_t* load, hipStream_t st);

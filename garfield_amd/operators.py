@@ -178,14 +178,15 @@ def mx_dequantise(w, dtype=None):
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(kind, t, M, rows, K):
+def _workspace_bytes(kind, off, t, M, ld, rows, K):
+    """off: the address modulo 16, all that the size needs of it."""
     n = C.c_size_t()
-    _lib._check(_lib.load().gf_mx_product_workspace(kind, t, M, rows, K, C.byref(n)))
+    _lib._check(_lib.load().gf_mx_product_workspace_at(kind, off, t, M, ld, rows, K, C.byref(n)))
     return n.value
 
 
-def _workspace(kind, t, M, w):
-    n = _workspace_bytes(kind, t, M, w.rows, w.K)
+def _workspace(kind, x, t, M, ld, w):
+    n = _workspace_bytes(kind, x.data_ptr() % 16, t, M, ld, w.rows, w.K)
     return (torch.empty(n, dtype=torch.uint8, device=w.device), n) if n else (None, 0)
 
 
@@ -209,7 +210,7 @@ def _product(x, w, dtype):
     dtype = dtype or x.dtype
     to = _type(dtype, "dtype")
     out = torch.empty((M, w.rows), dtype=dtype, device=w.device)
-    ws, nws = _workspace(0, t, M, w)
+    ws, nws = _workspace(0, x, t, M, ld, w)
     _call(w.device, lib.gf_mx_product, x.data_ptr(), t, M, ld, C.byref(w._struct), to, out.data_ptr(), w.rows,
           ws.data_ptr() if nws else None, nws)
     return out
@@ -226,7 +227,7 @@ def mx_product_grad(dy, w, dtype=None):
     dtype = dtype or dy.dtype
     to = _type(dtype, "dtype")
     dx = torch.empty((M, w.K), dtype=dtype, device=w.device)
-    ws, nws = _workspace(2, t, M, w)
+    ws, nws = _workspace(2, dy, t, M, ld, w)
     _call(w.device, _lib.load().gf_mx_product_grad, dy.data_ptr(), t, M, ld, C.byref(w._struct), to,
           dx.data_ptr(), w.K, ws.data_ptr() if nws else None, nws)
     return dx

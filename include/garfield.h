@@ -491,8 +491,9 @@ gf_status gf_mx_dequantise(const gf_mx_rows* w /*host*/, int32_t dtype, void* ou
 
 /* out[m][n] = sum over k of x[m][k] * w[n][k]: the scores of M queries
  * against w's rows.  x is real (M x w->K); its values enter unrounded,
- * whatever their type, and sums are fp32.  workspace: gf_mx_product_workspace
- * bytes (may be NULL where that is 0), aligned to 16. */
+ * whatever their type, and sums are fp32.  workspace: the bytes that
+ * gf_mx_product_workspace or gf_mx_product_workspace_at names (may be NULL
+ * where that is 0), aligned to 16. */
 gf_status gf_mx_product(const void* x, int32_t dtype, uint64_t M, uint64_t ldx, const gf_mx_rows* w /*host*/,
                         int32_t out_dtype, void* out, uint64_t ldo, void* workspace, size_t workspace_bytes,
                         void* stream);
@@ -506,10 +507,16 @@ gf_status gf_mx_product_grad(const void* dy, int32_t dtype, uint64_t M, uint64_t
                              int32_t out_dtype, void* dx, uint64_t ldo, void* workspace, size_t workspace_bytes,
                              void* stream);
 /* Workspace of the three calls above for M rows of x (or dy) against `rows`
- * rows of K values; kind 0 gf_mx_product, 1 gf_mx_product_mx, 2
- * gf_mx_product_grad; dtype as the call's (unused for kind 1).  Host only. */
+ * rows of K values, wherever x lies; kind 0 gf_mx_product, 1 gf_mx_product_mx,
+ * 2 gf_mx_product_grad; dtype as the call's (unused for kind 1).  Never more
+ * than 4 GiB + 64 MiB.  Host only. */
 gf_status gf_mx_product_workspace(int32_t kind, int32_t dtype, uint64_t M, uint64_t rows, uint32_t K,
                                   size_t* bytes /*host*/);
+/* The same for one call's x (or dy) and its row distance, and what that call
+ * insists on: less where bfloat16 rows are read in place (whole steps of 64
+ * values, ldx a multiple of 8, x aligned to 16 bytes).  x is not read. */
+gf_status gf_mx_product_workspace_at(int32_t kind, const void* x, int32_t dtype, uint64_t M, uint64_t ldx,
+                                     uint64_t rows, uint32_t K, size_t* bytes /*host*/);
 
 /* Routing of T queries (tokens) to k of E cells (experts) each.  An entry is
  * live when its logit, and its bias if there is one, is neither -inf nor NaN
