@@ -509,7 +509,8 @@ gf_status gf_mx_product_grad(const void* dy, int32_t dtype, uint64_t M, uint64_t
 /* Workspace of the three calls above for M rows of x (or dy) against `rows`
  * rows of K values, wherever x lies; kind 0 gf_mx_product, 1 gf_mx_product_mx,
  * 2 gf_mx_product_grad; dtype as the call's (unused for kind 1).  Never more
- * than 4 GiB + 64 MiB.  Host only. */
+ * than 4 GiB + 64 MiB, but not monotone in any size: fewer rows may need more,
+ * so ask for every size, not for the largest.  Host only. */
 gf_status gf_mx_product_workspace(int32_t kind, int32_t dtype, uint64_t M, uint64_t rows, uint32_t K,
                                   size_t* bytes /*host*/);
 /* The same for one call's x (or dy) and its row distance, and what that call
