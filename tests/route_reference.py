@@ -1,6 +1,6 @@
-"""Weights and gradients of a routing in 64 bits from logarithms of the scores,
-which no logit brings to zero, and bounds for the GPU's entry by entry.  numpy
-only; the choice (ids) is an input."""
+"""A routing in 64 bits over whole arrays (numpy only): the choice by sorting;
+weights and gradients of a choice from logarithms of the scores, which no logit
+brings to zero; and bounds for the GPU's entry by entry."""
 import numpy as np
 
 from operators_oracle import FMAX, ROUNDING
@@ -24,6 +24,30 @@ def _shares(x):
     x = x - top                             # first: a large top would swallow the sum's logarithm
     total = np.exp(x).sum(1, keepdims=True)
     return x - np.log(np.where(total > 0, total, 1.0))
+
+
+def choose(logits, k, bias=None, groups=1, keep_groups=None, group_score="max", score="softmax"):
+    """(ids (T, k), load (E,)): ties to the lower index, -1 where fewer are live."""
+    l, live = live_logits(logits, bias)
+    T, E = l.shape
+    key = l
+    if bias is not None or (groups > 1 and group_score == "top2"):
+        with np.errstate(over="ignore"):
+            s = 1 / (1 + np.exp(-l)) if score == "sigmoid" else np.exp(_shares(l))
+        key = np.where(live, s + (0.0 if bias is None else np.asarray(bias, np.float64)), -np.inf)
+    if groups > 1:
+        by = key.reshape(T, groups, E // groups)
+        rank = by.max(2)
+        if group_score == "top2" and E > groups:
+            second = np.partition(by, -2, axis=2)[:, :, -2]
+            rank = rank + np.where(second > -np.inf, second, 0.0)
+        kept = np.argsort(-rank, axis=1, kind="stable")[:, :groups if keep_groups is None else keep_groups]
+        keep = np.zeros((T, groups), bool)
+        keep[np.arange(T)[:, None], kept] = True
+        key = np.where(np.repeat(keep, E // groups, axis=1), key, -np.inf)
+    ids = np.argsort(-key, axis=1, kind="stable")[:, :k]
+    ids = np.where(np.take_along_axis(key, ids, 1) > -np.inf, ids, -1).astype(np.int32)
+    return ids, np.bincount(ids[ids >= 0], minlength=E).astype(np.int32)
 
 
 def _chosen(logits, ids, score, renormalise, bias):
@@ -71,16 +95,16 @@ def gradient(logits, ids, dweights, score="softmax", renormalise=True, scale=1.0
 
 
 def relative_error(logits, ids, bias=None):
-    """Of a weight, by row: a difference of logits is rounded by 2^-24 of itself,
-    the exponential makes that its relative error and adds two units in the last
-    place (2^-23), the sum of at most 1024 positive terms at most 16 more (16 or
-    64 lanes of at most 64 terms, added as a tree, each term as far off as the
-    weight: twice all of it), a division and two products three."""
+    """Of a weight, by row, in units of 2^-24 (half a unit in the last place): a
+    difference v of logits, its product with a rounded log2 e and the exponential
+    are off by at most 3 |v| + 4, in the term and again in the sum of its row;
+    that sum is of at most 64 terms a lane, one after the other, and 6 exchanges;
+    a division and two products make 4 more."""
     l, live = live_logits(logits, bias)
-    with np.errstate(invalid="ignore"):
-        span = np.where(live, l, l.max(1, keepdims=True)).max(1) - np.where(live, l, np.inf).min(1)
-    span = np.minimum(np.where(live.any(1), span, 0.0), 120.0)        # beyond, e^-span is below 2^-149 anyway
-    return (2 * (span * 2.0 ** -24 + 2 * 2.0 ** -23) + (16 + 3) * 2.0 ** -23)[:, None]
+    low = np.where(live, l, np.inf).min(1)
+    span = np.where(live.any(1), l.max(1), 0.0) - np.where(live.any(1), low, 0.0)
+    span = np.minimum(span, 120.0)        # beyond, e^-span is below 2^-149 anyway
+    return ((2 * (3 * span + 4) + 64 + 6 + 4) * 2.0 ** -24)[:, None]
 
 
 def weight_bound(ref, logits, ids, scale, bias=None):

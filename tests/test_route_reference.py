@@ -53,3 +53,15 @@ def test_gradient_against_differences(score, low):
 def test_shares_of_low_sigmoids():
     w = ref.weights(np.array([[-100.0, -101.0]]), np.array([[0, 1]]), score="sigmoid")
     assert np.allclose(w, [[1 / (1 + np.exp(-1)), 1 / (1 + np.exp(1))]], rtol=1e-12)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,keep,rank", [(1, 1, "max"), (6, 2, "max"), (6, 2, "top2"), (12, 5, "top2"), (6, 6, "top2")])
+def test_choice_agrees_with_the_oracle(groups, keep, rank, score):
+    rng = np.random.default_rng(groups)
+    l, _, _ = _case(60, 12, 4, 5)
+    l[20:40] = np.round(l[20:40])
+    for bias in (None, 0.1 * rng.standard_normal(12), np.array([0.25] * 11 + [-np.inf])):
+        want = orc.route(l, 2, bias=bias, groups=groups, keep_groups=keep, group_score=rank, score=score)
+        got = ref.choose(l, 2, bias, groups, keep, rank, score)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[2])
