@@ -65,3 +65,27 @@ def test_choice_agrees_with_the_oracle(groups, keep, rank, score):
         want = orc.route(l, 2, bias=bias, groups=groups, keep_groups=keep, group_score=rank, score=score)
         got = ref.choose(l, 2, bias, groups, keep, rank, score)
         assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[2])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("E,k", [(16, 2), (64, 8), (256, 8), (1024, 16), (1024, 64)])
+def test_gradient_bound_sees_a_lost_term(E, k, dtype):
+    """Softmax over all entries: a gradient without the term of the entries that
+    were not chosen, or with it a hundredth off, is outside the bound."""
+    l, ids, g = _case(30, E, k, E + k, masked=False)
+    how = dict(renormalise=False, scale=2.5)
+    d, mag = ref.gradient(l, ids, g, **how)
+    bound = ref.gradient_bound(d, mag, l, ids, g, 2.5, dtype)
+    other = np.ones(l.shape, bool)
+    np.put_along_axis(other, ids, False, 1)
+    # what a type's own least value swallows cannot be seen in it
+    seen = other & (np.abs(d) > 4 * orc.ROUNDING[dtype][1])
+    assert seen.sum() > 0.9 * other.sum()
+    # entries whose average of gradients nearly vanishes have little to lose
+    assert (np.abs(d) > bound)[seen].mean() > 0.99
+    if dtype == "float32":
+        assert (np.abs(0.01 * d) > bound)[seen].mean() > 0.9
+    # the bound that is absolute in the largest gradient lets the lost term pass at the largest size
+    loose = orc.grad_bound(d, g, 2.5, dtype)
+    if (E, k) == (1024, 64):
+        assert (np.abs(d) <= loose)[other].all()
