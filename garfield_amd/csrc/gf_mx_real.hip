@@ -1,10 +1,12 @@
 // Products of real rows with 4-bit rows, and their gradient, on the bfloat16
 // matrix instructions.
 //
-// A value of a 4-bit row is exact in bfloat16, whose exponent range is the
-// format's, so only the real side could lose bits.  It does not: a binary16
-// value is the sum of two bfloat16 values, an fp32 value of three (truncated
-// eight bits at a time), and the product runs once over each of these planes.
+// A value of a 4-bit row is exact in bfloat16 at scale bytes up to 252 (at 253 and
+// 254, which quantisation never writes, codes from 4 and 2 on become infinities),
+// so only the real side could lose bits.  It does not: a binary16 value is the sum
+// of two bfloat16 values, an fp32 value of three (truncated eight bits at a time;
+// what lies below bfloat16's least, 2^-133, is cut off), and the product runs once
+// over each of these planes.
 #include <algorithm>
 
 #include "gf_mx_device.h"

@@ -96,7 +96,9 @@ def _call(device, fn, *args):
 
 class MXRows:
     """Rows at four bits: codes (rows, 64 S) and scales (rows, 4 S), uint8,
-    S = ceil(K / 128); the layout is gf_mx_rows'."""
+    S = ceil(K / 128); the layout is gf_mx_rows'.  Scale bytes of 253 and 254,
+    which mx_quantise never writes, hold values beyond fp32 and bfloat16: only
+    the product with both sides at four bits takes them."""
 
     def __init__(self, codes, scales, K):
         _need_torch()

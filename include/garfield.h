@@ -471,7 +471,11 @@ gf_status gf_quantise_i8(const float* x, uint64_t n, uint32_t D, float alpha, fl
  * codes 64 S bytes from codes + r * 64 S, two a byte, the even element in the
  * low half, and scales 4 S bytes from scales + r * 4 S.  Values beyond K are
  * code 0, blocks wholly beyond K have scale byte 0: the products read whole
- * chunks and rely on it.  codes must be aligned to 16 bytes, scales to 4. */
+ * chunks and rely on it.  Scale bytes 253 and 254, which gf_mx_quantise never
+ * writes, make the larger codes pass fp32's and bfloat16's range:
+ * gf_mx_product_mx takes them at their value, gf_mx_dequantise gives infinities,
+ * and a product with real rows or its gradient gives infinities or NaN where
+ * such values enter, whatever they are multiplied by.  codes must be aligned to 16 bytes, scales to 4. */
 typedef struct {
     const uint8_t* codes;
     const uint8_t* scales;
@@ -491,7 +495,8 @@ gf_status gf_mx_dequantise(const gf_mx_rows* w /*host*/, int32_t dtype, void* ou
 
 /* out[m][n] = sum over k of x[m][k] * w[n][k]: the scores of M queries
  * against w's rows.  x is real (M x w->K); its values enter unrounded,
- * whatever their type, and sums are fp32.  workspace: the bytes that
+ * whatever their type (of an fp32 value down to 2^-133: bits below that are
+ * cut off), and sums are fp32.  workspace: the bytes that
  * gf_mx_product_workspace or gf_mx_product_workspace_at names (may be NULL
  * where that is 0), aligned to 16. */
 gf_status gf_mx_product(const void* x, int32_t dtype, uint64_t M, uint64_t ldx, const gf_mx_rows* w /*host*/,
