@@ -12,8 +12,11 @@ namespace {
 // (V = 4 or 8 values), so 8 or 4 lanes share a block and 32 or 16 a chunk of
 // 128 values; kAhead chunks a lane are loaded before the first is used.  1M x
 // 128: fp32 96 us to codes (6.1 TB/s; 105 with loads that stay in the caches),
-// bfloat16 52 us (61 with one chunk ahead); back 115 and 90 us (141 and 92 with
-// one chunk ahead, 115 and 99 with four).
+// bfloat16 52 us (61 with one chunk ahead); back in turn with quantisations 115 and
+// 90 us (141 and 92 with one chunk ahead, 115 and 99 with four), by itself 148 and
+// 85, binary16 87: 3.7 to 3.9 TB/s, where a fill of the same bytes takes 78 and 40.
+// Rows that are not whole chunks of 16-byte pieces share lines: 1M x 130 235 us in
+// fp32, 2.8 TB/s, 135 in bfloat16.
 
 template <bool BACK>
 constexpr uint32_t kAhead = BACK ? 2 : 4;

@@ -217,10 +217,11 @@ __global__ __launch_bounds__(64 * WK) void k_mx_few(const ElemT<DT>* x, uint32_t
 // The sum may be cut into `parts`, each block then writing its own in fp32 to
 // a workspace (out, rows of ldo, a part every M ldo), which k_mx_join adds up
 // in order.
-// 4096 x 8192 x 4096 in bfloat16 takes 215 us by tiles of 256, 1.28 PFLOP/s where the
-// library's product of two bfloat16 matrices reaches 1.40 at 8192 x 8192 x 8192, the
-// gradient 222; the matrix cores are busy for 45% of the cycles, at what the
-// chip's power leaves of the clock.
+// 4096 x 8192 x 4096 in bfloat16 takes 222 us by tiles of 256 where calls follow one
+// another (215 to 225 by the card), 1.24 PFLOP/s where the library's product of two
+// bfloat16 matrices reaches 1.40 at 8192 x 8192 x 8192, the gradient 222 too; a call
+// by itself 245, most under the profiler 235 to 258.  The matrix cores are busy for
+// 45% of the cycles, at what the chip's power leaves of the clock.
 template <int DT, bool COPIED, int BM, int BN, int OT, bool TR>
 struct RealLds {
     static_assert(DT == GF_BF16 || !COPIED, "");
@@ -519,7 +520,7 @@ uint32_t planes_of(int32_t dtype) { return dtype == GF_BF16 ? 1u : dtype == GF_F
 // the smaller ones) and once what a tile takes besides; a launch and 7 TB/s for
 // planes and for joining parts, which are read back from the caches for the most
 // part.  Fitted to 240 products and gradients of 17 to 10,000 real rows with each
-// tile: five in six of its times are within 15% of the measured one, and the
+// tile: four in five of its times are within 15% of the measured one, and the
 // tile it takes was 1% slower than the best on average and 18% at most.  Parts up
 // to one block a unit instead: the gradient of 4077 rows in fp32 over 5678 rows of
 // 365 93 us against 75, 2759 over 31907 of 514 508 against 421.  Large,

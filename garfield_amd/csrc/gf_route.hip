@@ -425,10 +425,17 @@ __device__ __forceinline__ void join_row(double* a, bool want_rest, double& rest
 // that are whole lanes are ranked from the lanes' two best, by moves between
 // lanes; others through LDS.
 //
-// What bounds it is the instructions issued, not the bytes read: 10,000 rows of
-// 256 in 32 bits, k = 8 by logit, 4 of 16 groups kept, take 15 us with the load and
-// the launch that clears it (21 by the loop), 16,384 rows by sigmoid and bias in 8
-// groups 23 us (30); what they read takes 2 and 4.  A whole wave for a row of more
+// What bounds it is a row's chain of dependent steps in few waves, and how the
+// blocks share the chip, not the bytes: 10,000 rows of 256 in 32 bits, k = 8 by
+// logit, 4 of 16 groups kept, take 13 us and the launch that clears the load 1.4
+// (21 by the loop), 16,384 rows by sigmoid and bias in 8 groups 22 (30); what they
+// read takes 2 and 4.  The vector instructions (296 and 390 a row) would take 5
+// and 10 spread over all compute units; waves wait for half of their cycles.  A
+// unit holds one block of sixteen waves, which takes about as long whether others
+// run or not: by logit 8192 rows (128 blocks) take 12.7 us, 16,384 (256) 15.2,
+// 20,000 (313, two rounds) 24.  Blocks of sixteen waves hold every instance to 128
+// registers: of some, 4 to 28 go to scratch (13 of lists of 16 at 256 entries).
+// A whole wave for a row of more
 // than 256 (8 or 16 entries a lane instead of 32 or 64, a quarter of the
 // registers) took 28 us for 4 rows of 1008 where sixteen lanes took 71, 62 for
 // 10,636 rows of 1018 where they took 73.
@@ -503,7 +510,10 @@ __global__ __launch_bounds__(1024) void k_route(gf_route_opts o, const T* logits
         // bound of s may stand for it, |k| + top or 1.  Sigmoid: the error of
         // e = e^-v weighs e / (1 + e)^2, below 1/4, which |v| times is below 0.23: 2^-24
         // in all; the sum, the reciprocal (2^-23) and the sum with the bias add 2^-22 of
-        // the score and the key.
+        // the score and the key.  An infinite bias makes every bound of its row infinite, and
+        // sigmoids around 2^-24 and below are all within theirs: such rows go through
+        // the pass in 64 bits (16,384 x 256, 8 groups by two best: 30 us, with one
+        // infinite bias 79, with all logits near -30 87).
         auto off = [&](float k) {
             const float u = fabsf(k) + top, s = fminf(u, 1.0f);
             return soft ? 0x1p-23f * (s * (14.0f + V / 2 - 0.6931472f * __builtin_amdgcn_logf(s + 0x1p-126f)) + u) + 0x1p-126f
@@ -759,8 +769,10 @@ __global__ void k_route_clear(int32_t* load, uint32_t E) {
 // put into a row of LDS that is written out whole; the softmax over all
 // entries adds its term to every live one.  16,384 rows of 256 in 32 bits, 8
 // chosen: 7 us, 2.4 TB/s of gradient, bound by the chain from ids over logits to
-// the sums; 15,287 rows of 992 with the softmax over all 74 us (177 with each
-// exponential taken twice), bound by the exponentials.
+// the sums; 15,287 rows of 992 with the softmax over all 57 us, 2.1 TB/s read and
+// written, where the vector instructions would take 13: a block's 63.5 KB of LDS
+// leave two waves a SIMD, which wait for 72% of their cycles.  Each exponential is
+// taken once (twice took 2.4 times as long).
 constexpr uint32_t kGradWaves = 4, kGradRows = 4;   // a block's waves, a wave's rows
 template <class T>
 __global__ __launch_bounds__(64 * kGradWaves) void k_route_grad(gf_route_opts o, const T* logits, uint32_t rows, uint32_t E,
